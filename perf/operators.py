@@ -297,7 +297,8 @@ def held_in_8_bits(x):
     b = torch.nn.functional.pad(x, (0, -C % BLOCK)).unflatten(-1, (-1, BLOCK))
     top = b.abs().amax(-1, keepdim=True)
     none = top < TINY
-    inv = torch.where(none, torch.zeros_like(top), 127.0 / torch.where(none, torch.ones_like(top), top))
+    # tensor by tensor: a number divided by a tensor would be its reciprocal times the number, rounded twice
+    inv = torch.where(none, torch.zeros_like(top), torch.full_like(top, 127.0) / torch.where(none, torch.ones_like(top), top))
     scale = torch.where(none, torch.zeros_like(top), top / 127.0)
     return (torch.round(b * inv) * scale).flatten(-2)[..., :C]
 
