@@ -317,6 +317,88 @@ int wubu_b200_disc_launches(const WubuB200Disc* d); /* kernels the last step / g
 int wubu_b200_disc_attach_comm(WubuB200Disc* d, int rank, int world, const void* id128);
 int wubu_b200_disc_set_comm_timeout_ms(WubuB200Disc* d, int ms);
 
+/* ---------------------------------------------------------------------------------------------
+ * 4. Transformer training operators (wubu_b200_act8_*, _resnorm_*): what the layers of a
+ *    self-attention encoder in front of the generator are made of, besides their matrix products.
+ *    Device pointers; every call enqueues on `stream` (cudaStream_t or NULL) of the current device
+ *    and returns without synchronising.  Arguments are checked before anything is launched
+ *    (WUBU_B200_ERR_ARG: a missing pointer, a bad enum, stride or alignment; WUBU_B200_ERR_SHAPE: a
+ *    size that the operator does not take; WUBU_B200_ERR_NOMEM: a workspace that is too small).
+ *    Results are reproducible bit for bit.
+ * ------------------------------------------------------------------------------------------- */
+#define WUBU_B200_F32 0
+#define WUBU_B200_BF16 1
+#define WUBU_B200_F16 2
+
+/* Waits for `stream` and reports the operators' device status: WUBU_B200_ERR_TIMEOUT once after a
+ * bounded wait inside one of their kernels expired on this device (what that call wrote is then
+ * unspecified), WUBU_B200_ERR_CUDA for a CUDA error, else 0. */
+int wubu_b200_ops_sync(void* stream);
+
+/* Activation with an 8-bit checkpoint of its input.
+ *   forward:  y = act(x); x is kept as q (int8) with one fp32 scale per block of 128 consecutive
+ *             values of a row (the last block of a row may be shorter): scale = max|x| / 127,
+ *             q = round-to-even(x * (127 / max|x|)).  A block whose max|x| is below 2^-100 is kept
+ *             as zeros; a block that holds an infinity or a NaN gets scale NaN, and all of it is
+ *             restored as NaN.
+ *   backward: with x' = q * scale, dx = dy * act'(x') and, where asked for, y' = act(x') (what the
+ *             next layer's weight gradient reads, so that y need not be kept either).
+ * act: WUBU_B200_ACT_*; slope: of the leaky ReLU (0 = ReLU), whose derivative at 0 is the slope.
+ * x, dy: `rows` rows of `cols` values, row strides in elements; y, q, dx, y_again: contiguous rows;
+ * scale: [rows][ceil(cols / 128)].  y may be NULL (checkpoint only); dy and dx may both be NULL
+ * (y_again only: with WUBU_B200_ACT_IDENTITY this restores x'). */
+#define WUBU_B200_ACT_IDENTITY 0
+#define WUBU_B200_ACT_LRELU 1
+#define WUBU_B200_ACT_GELU 2 /* x * Phi(x), the error-function form */
+#define WUBU_B200_ACT_SILU 3
+int wubu_b200_act8_forward(int dtype, int act, float slope, const void* x, long long x_stride, void* y, signed char* q,
+                           float* scale, long long rows, int cols, void* stream);
+int wubu_b200_act8_backward(int dtype, int act, float slope, const void* dy, long long dy_stride, const signed char* q,
+                            const float* scale, void* dx, void* y_again, long long rows, int cols, void* stream);
+
+/* The norms around a block, its gate and the residual scale, in one pass:
+ *     u = post(f),  r = res_scale * x + gate * u,  h = norm(r)
+ * norm / post: WUBU_B200_NORM_* over the row: (v - mean) / sqrt(var + eps) * weight + bias, or
+ * v / sqrt(mean(v^2) + eps) * weight, or none (u = f; no h).  gate: none (1), one value per column,
+ * or one per item and column.  h is formed from the unrounded r.  Rows are items * rows_per_item; x,
+ * f, dr and dh have row strides in elements; r, h, dx and df are contiguous.  Statistics, sums and
+ * all parameter vectors are fp32.  cols: 1 to 8192.
+ * backward: from dr (gradient of r, NULL = 0) and dh (gradient of h, NULL = 0) it recomputes u, r and
+ * both norms from x and f and writes dx, df and the sums over rows dgate ([cols] or
+ * [items][cols]), dpost_weight, dpost_bias, dweight and dbias; any of the outputs may be NULL.
+ * The workspace holds partial column sums: wubu_b200_resnorm_workspace bytes, none in the forward. */
+#define WUBU_B200_NORM_NONE 0
+#define WUBU_B200_NORM_LAYER 1
+#define WUBU_B200_NORM_RMS 2
+#define WUBU_B200_GATE_NONE 0
+#define WUBU_B200_GATE_COLUMN 1
+#define WUBU_B200_GATE_ITEM 2
+typedef struct WubuB200ResNorm {
+  int dtype, norm, post, gate;
+  long long items, rows_per_item;
+  int cols;
+  float res_scale, eps;
+  int reserved;
+  const void* x;
+  long long x_stride;
+  const void* f;
+  long long f_stride;
+  const float *weight, *bias, *post_weight, *post_bias; /* NULL: ones / zeros */
+  const float* gate_values;
+  void *r, *h; /* forward; NULL = not written */
+  const void* dr;
+  long long dr_stride;
+  const void* dh;
+  long long dh_stride;
+  void *dx, *df;
+  float *dgate, *dpost_weight, *dpost_bias, *dweight, *dbias;
+  void* workspace;
+  long long workspace_bytes;
+} WubuB200ResNorm;
+int wubu_b200_resnorm_forward(const WubuB200ResNorm* a, void* stream);
+long long wubu_b200_resnorm_workspace(const WubuB200ResNorm* a); /* of the backward; negative = error */
+int wubu_b200_resnorm_backward(const WubuB200ResNorm* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

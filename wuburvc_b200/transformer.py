@@ -1,0 +1,291 @@
+"""Transformer training operators on the native library (section 4 of include/wuburvc_b200.h), for
+torch CUDA tensors: what the layers of a self-attention encoder in front of the generator are made of,
+besides their matrix products.
+
+* ``act8_forward`` / ``act8_backward``: an activation whose input is kept in 8 bits for the backward;
+* ``resnorm_forward`` / ``resnorm_backward``: the norms around a block, its gate and the residual scale.
+
+Calls enqueue on the current torch stream of the tensors' device and do not synchronise; outputs are new
+tensors.  A call that cannot be made raises (``ValueError`` for its arguments, ``RuntimeError`` for a
+code of the library); there is no fallback to torch.  Last dimensions are contiguous (others are copied
+first); ``ops_sync`` reports what an asynchronous call could not.
+"""
+from __future__ import annotations
+
+import ctypes
+import struct
+from typing import NamedTuple
+
+import torch
+
+from ._lib import lib
+
+_vp, _ip, _fp, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
+_SIGS = {
+    "wubu_b200_ops_sync": (_ip, [_vp]),
+    "wubu_b200_act8_forward": (_ip, [_ip, _ip, _fp, _vp, _ll, _vp, _vp, _vp, _ll, _ip, _vp]),
+    "wubu_b200_act8_backward": (_ip, [_ip, _ip, _fp, _vp, _ll, _vp, _vp, _vp, _vp, _ll, _ip, _vp]),
+    "wubu_b200_resnorm_forward": (_ip, [ctypes.c_char_p, _vp]),
+    "wubu_b200_resnorm_workspace": (_ll, [ctypes.c_char_p]),
+    "wubu_b200_resnorm_backward": (_ip, [ctypes.c_char_p, _vp]),
+}
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ACTS = {"identity": 0, "lrelu": 1, "gelu": 2, "silu": 3}
+_NORMS = {None: 0, "layer": 1, "rms": 2}
+ACT8_BLOCK = 128
+_bound = None
+
+
+def L():
+    global _bound
+    if _bound is None:
+        h = lib()
+        for name, (res, args) in _SIGS.items():
+            f = getattr(h, name)
+            f.restype = res
+            f.argtypes = args
+        _bound = h
+    return _bound
+
+
+def _check(rc, what):
+    if rc < 0:
+        raise RuntimeError(f"wuburvc_b200 {what} failed with code {rc}")
+    return rc
+
+
+def _dtype(t, what):
+    d = _DTYPES.get(t.dtype)
+    if d is None:
+        raise ValueError(f"{what}: float32, bfloat16 or float16 tensors, got {t.dtype}")
+    return d
+
+
+def _cuda(what, *ts):
+    dev = ts[0].device
+    if dev.type != "cuda":
+        raise ValueError(f"{what}: CUDA tensors only")
+    for t in ts[1:]:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+    return dev
+
+
+class _on:
+    """The library launches on the current device: makes ``dev`` current where it is not."""
+
+    def __init__(self, dev):
+        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *e):
+        if self.guard is not None:
+            self.guard.__exit__(*e)
+
+
+def _stream(dev):
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _rows(t):
+    """(t, row stride) of a tensor seen as rows of its last dimension: a view where one row stride
+    describes it, else a copy."""
+    C = t.shape[-1]
+    if t.is_contiguous():
+        return t, C
+    if t.dim() and t.stride(-1) == 1 or C == 1:
+        step = None
+        want = None
+        for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if n == 1:
+                continue
+            if step is None:
+                step, want = s, s * n
+            elif s != want:
+                step = None
+                break
+            else:
+                want = s * n
+        if step is not None and step >= C and (C == 1 or t.stride(-1) == 1):
+            return t, step
+    t = t.contiguous()
+    return t, C
+
+
+def ops_sync(device=None):
+    """Waits for the current stream and raises if a kernel of these operators gave up on a wait."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    with _on(dev):
+        _check(L().wubu_b200_ops_sync(_stream(dev)), "ops_sync")
+
+
+# ---- activation with an 8-bit checkpoint of its input --------------------------------------------
+
+
+class Kept8(NamedTuple):
+    """What ``act8_forward`` keeps of its input: int8 values and a scale per 128 values of a row."""
+
+    q: torch.Tensor
+    scale: torch.Tensor
+    act: str
+    slope: float
+    dtype: torch.dtype
+
+
+def act8_forward(x, act="gelu", slope=0.0, with_output=True):
+    """``(act(x), kept)``; ``kept`` is what ``act8_backward`` reads in place of x.  ``act``: "lrelu"
+    (with ``slope``; 0 is the ReLU), "gelu", "silu" or "identity".  ``with_output=False`` only keeps x."""
+    d = _dtype(x, "act8_forward")
+    if act not in _ACTS:
+        raise ValueError(f"act8_forward: act is one of {sorted(_ACTS)}, got {act!r}")
+    if x.dim() < 1:
+        raise ValueError("act8_forward: x has a last dimension")
+    dev = _cuda("act8_forward", x)
+    x, step = _rows(x)
+    C = x.shape[-1]
+    rows = x.numel() // C if C else 0
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev) if with_output else None
+    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
+    scale = torch.empty((*x.shape[:-1], -(-C // ACT8_BLOCK)), dtype=torch.float32, device=dev)
+    with _on(dev):
+        _check(L().wubu_b200_act8_forward(d, _ACTS[act], slope, x.data_ptr(), step, _ptr(y), q.data_ptr(),
+                                          scale.data_ptr(), rows, C, _stream(dev)), "act8_forward")
+    return y, Kept8(q, scale, act, float(slope), x.dtype)
+
+
+def act8_backward(dy, kept, recompute=False):
+    """``(dx, y)`` from the kept form x' of x: dx = dy act'(x'); y = act(x') if ``recompute``, else
+    None.  ``dy=None`` gives ``(None, act(x'))`` alone."""
+    q, scale = kept.q, kept.scale
+    if dy is not None and (dy.shape != q.shape or dy.dtype != kept.dtype):
+        raise ValueError(f"act8_backward: dy is {tuple(q.shape)} {kept.dtype}, got {tuple(dy.shape)} {dy.dtype}")
+    dev = _cuda("act8_backward", q, scale, dy)
+    C = q.shape[-1]
+    rows = q.numel() // C if C else 0
+    step, dx, y = 0, None, None
+    if dy is not None:
+        dy, step = _rows(dy)
+        dx = torch.empty(q.shape, dtype=kept.dtype, device=dev)
+    if recompute or dy is None:
+        y = torch.empty(q.shape, dtype=kept.dtype, device=dev)
+    with _on(dev):
+        _check(L().wubu_b200_act8_backward(_DTYPES[kept.dtype], _ACTS[kept.act], kept.slope, _ptr(dy), step,
+                                           q.data_ptr(), scale.data_ptr(), _ptr(dx), _ptr(y), rows, C, _stream(dev)),
+               "act8_backward")
+    return dx, y
+
+
+def act8_restore(kept):
+    """The kept form of x itself, in x's type."""
+    return act8_backward(None, kept._replace(act="identity"), recompute=True)[1]
+
+
+# ---- norms around a block, gate and residual scale ------------------------------------------------
+
+_RESNORM = struct.Struct("@4i2qi2fi" + "4q" + "4P" + "P" + "2P" + "4q" + "2P" + "5P" + "Pq")
+
+
+def _vector(v, shape, dev, what):
+    if v is None:
+        return None
+    if tuple(v.shape) != shape:
+        raise ValueError(f"{what}: shape {shape}, got {tuple(v.shape)}")
+    if v.device != dev:
+        raise ValueError(f"{what}: tensors on {dev} and {v.device}")
+    if v.dtype != torch.float32 or not v.is_contiguous():
+        v = v.to(torch.float32).contiguous()
+    return v
+
+
+def _resnorm_operands(what, x, f, norm, weight, bias, post, post_weight, post_bias, gate):
+    if x.dim() < 2 or f.shape != x.shape or f.dtype != x.dtype:
+        raise ValueError(f"{what}: x and f are [items, ..., cols] of one shape and type")
+    if norm not in _NORMS or post not in _NORMS:
+        raise ValueError(f"{what}: norm and post are None, 'layer' or 'rms'")
+    if (bias is not None and norm != "layer") or (post_bias is not None and post != "layer"):
+        raise ValueError(f"{what}: only a layer norm has a bias")
+    if (weight is not None and norm is None) or (post_weight is not None and post is None):
+        raise ValueError(f"{what}: a weight without its norm")
+    dev = _cuda(what, x, f)
+    items, C = x.shape[0], x.shape[-1]
+    rows = x.numel() // (items * C) if items and C else 0
+    vec = [_vector(v, (C,), dev, what + " " + n) for v, n in
+           ((weight, "weight"), (bias, "bias"), (post_weight, "post_weight"), (post_bias, "post_bias"))]
+    kind = 0
+    if gate is not None:
+        kind = 1 if gate.dim() == 1 else 2
+        gate = _vector(gate, (C,) if kind == 1 else (items, C), dev, what + " gate")
+    return dev, items, rows, C, vec, kind, gate
+
+
+def resnorm_forward(x, f, *, norm="layer", weight=None, bias=None, post=None, post_weight=None, post_bias=None,
+                    gate=None, res_scale=1.0, eps=1e-5, keep_sum=True):
+    """``(r, h)`` with r = res_scale * x + gate * post(f) and h = norm(r), for x, f ``[items, ..., cols]``.
+
+    ``norm`` / ``post``: "layer", "rms" or None, with ``weight`` / ``bias`` and ``post_weight`` /
+    ``post_bias`` of ``[cols]`` (None: ones / zeros; RMS norms have no bias).  ``gate``: None,
+    ``[cols]`` or ``[items, cols]``.  ``keep_sum=False`` returns None for r; ``norm=None`` None for h."""
+    d = _dtype(x, "resnorm_forward")
+    dev, items, rows, C, vec, kind, gate = _resnorm_operands("resnorm_forward", x, f, norm, weight, bias, post,
+                                                             post_weight, post_bias, gate)
+    x, xs = _rows(x)
+    f, fs = _rows(f)
+    r = torch.empty(x.shape, dtype=x.dtype, device=dev) if keep_sum else None
+    h = torch.empty(x.shape, dtype=x.dtype, device=dev) if norm else None
+    args = _RESNORM.pack(d, _NORMS[norm], _NORMS[post], kind, items, rows, C, res_scale, eps, 0, x.data_ptr(), xs,
+                         f.data_ptr(), fs, *map(_ptr, vec), _ptr(gate), _ptr(r), _ptr(h), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                         0, 0, 0)
+    with _on(dev):
+        _check(L().wubu_b200_resnorm_forward(args, _stream(dev)), "resnorm_forward")
+    return r, h
+
+
+def resnorm_backward(dr, dh, x, f, *, norm="layer", weight=None, bias=None, post=None, post_weight=None,
+                     post_bias=None, gate=None, res_scale=1.0, eps=1e-5):
+    """Gradients of ``resnorm_forward`` for the gradients ``dr`` of r and ``dh`` of h (either may be
+    None): a dict of dx, df, dgate, dweight, dbias, dpost_weight, dpost_bias, None for what the
+    operator was not given.  The vectors' gradients are float32 sums over the rows."""
+    what = "resnorm_backward"
+    d = _dtype(x, what)
+    dev, items, rows, C, vec, kind, gate = _resnorm_operands(what, x, f, norm, weight, bias, post, post_weight,
+                                                             post_bias, gate)
+    strides = [0, 0]
+    grads = [dr, dh]
+    for i, t in enumerate(grads):
+        if t is None:
+            continue
+        if t.shape != x.shape or t.dtype != x.dtype or t.device != dev:
+            raise ValueError(f"{what}: dr and dh have x's shape, type and device")
+        grads[i], strides[i] = _rows(t)
+    if dr is None and dh is None:
+        raise ValueError(f"{what}: dr or dh is needed")
+    if dh is not None and norm is None:
+        raise ValueError(f"{what}: dh without a norm")
+    dr, dh = grads
+    x, xs = _rows(x)
+    f, fs = _rows(f)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    df = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    like = lambda v: None if v is None else torch.empty(v.shape, dtype=torch.float32, device=dev)  # noqa: E731
+    dweight, dbias, dpost_weight, dpost_bias, dgate = (like(v) for v in (*vec, gate))
+
+    def pack(ws, n):
+        return _RESNORM.pack(d, _NORMS[norm], _NORMS[post], kind, items, rows, C, res_scale, eps, 0, x.data_ptr(), xs,
+                             f.data_ptr(), fs, *map(_ptr, vec), _ptr(gate), 0, 0, _ptr(dr), strides[0], _ptr(dh),
+                             strides[1], dx.data_ptr(), df.data_ptr(), _ptr(dgate), _ptr(dpost_weight),
+                             _ptr(dpost_bias), _ptr(dweight), _ptr(dbias), ws, n)
+
+    h = L()
+    with _on(dev):
+        n = _check(h.wubu_b200_resnorm_workspace(pack(0, 0)), what)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        _check(h.wubu_b200_resnorm_backward(pack(ws.data_ptr(), n), _stream(dev)), what)
+    return {"dx": dx, "df": df, "dgate": dgate, "dweight": dweight, "dbias": dbias, "dpost_weight": dpost_weight,
+            "dpost_bias": dpost_bias}
