@@ -318,7 +318,7 @@ int wubu_b200_disc_attach_comm(WubuB200Disc* d, int rank, int world, const void*
 int wubu_b200_disc_set_comm_timeout_ms(WubuB200Disc* d, int ms);
 
 /* ---------------------------------------------------------------------------------------------
- * 4. Transformer training operators (wubu_b200_act8_*, _resnorm_*): what the layers of a
+ * 4. Transformer training operators (wubu_b200_act8_*, _resnorm_*, _attn_*): what the layers of a
  *    self-attention encoder in front of the generator are made of, besides their matrix products.
  *    Device pointers; every call enqueues on `stream` (cudaStream_t or NULL) of the current device
  *    and returns without synchronising.  Arguments are checked before anything is launched
@@ -398,6 +398,38 @@ typedef struct WubuB200ResNorm {
 int wubu_b200_resnorm_forward(const WubuB200ResNorm* a, void* stream);
 long long wubu_b200_resnorm_workspace(const WubuB200ResNorm* a); /* of the backward; negative = error */
 int wubu_b200_resnorm_backward(const WubuB200ResNorm* a, void* stream);
+
+/* Softmax attention and its gradient, the probabilities recomputed from the log-sum-exp:
+ *     S = scale * Q K^T,  P = softmax over the visible keys,  O = P V,  lse = log sum exp S
+ * over views [B][T][H][D] with any batch, token and head strides (in elements; the last dimension
+ * is contiguous).  Hq is a multiple of Hkv: query head h reads key / value head h / (Hq / Hkv), and dk,
+ * dv sum over the query heads that share one.  q_lens / k_lens (device int32 [B], NULL = Tq / Tk)
+ * give each item's length: what lies beyond is neither read into a result nor differentiated, and
+ * may hold anything.  Query i sits at place p = i + k_len - q_len among the keys; key j is visible
+ * if j < k_len, and j <= p (causal), and |p - j| < window (window > 0).  A query that sees no key,
+ * or lies beyond q_len, has O = 0, lse = -infinity and no gradient; dk, dv beyond k_len are 0.
+ * dtype: WUBU_B200_BF16 or _F16.  D: a multiple of 8, 8 to 128.  Every pointer is aligned to 16 bytes
+ * and every stride is a multiple of 8 elements.  lse: fp32 [B][Hq][Tq].  scale: 0 = 1 / sqrt(D).
+ * The forward reads q, k, v and writes out, lse; the backward reads those five and dout and writes
+ * dq, dk, dv.  Scores, softmax statistics and all sums are fp32; P and dS enter their matrix
+ * products in the inputs' type.  The workspace is wubu_b200_attn_workspace bytes (may be 0). */
+typedef struct WubuB200View {
+  void* data;
+  long long batch, token, head; /* strides in elements */
+} WubuB200View;
+typedef struct WubuB200Attn {
+  int dtype, B, Hq, Hkv, Tq, Tk, D, causal, window;
+  float scale;
+  const int *q_lens, *k_lens;
+  WubuB200View q, k, v, out;
+  float* lse;
+  WubuB200View dout, dq, dk, dv;
+  void* workspace;
+  long long workspace_bytes;
+} WubuB200Attn;
+long long wubu_b200_attn_workspace(const WubuB200Attn* a, int backward); /* negative = error */
+int wubu_b200_attn_forward(const WubuB200Attn* a, void* stream);
+int wubu_b200_attn_backward(const WubuB200Attn* a, void* stream);
 
 #ifdef __cplusplus
 }

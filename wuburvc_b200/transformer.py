@@ -3,7 +3,9 @@ torch CUDA tensors: what the layers of a self-attention encoder in front of the 
 besides their matrix products.
 
 * ``act8_forward`` / ``act8_backward``: an activation whose input is kept in 8 bits for the backward;
-* ``resnorm_forward`` / ``resnorm_backward``: the norms around a block, its gate and the residual scale.
+* ``resnorm_forward`` / ``resnorm_backward``: the norms around a block, its gate and the residual scale;
+* ``attention_forward`` / ``attention_backward``: softmax attention, its gradient with the probabilities
+  recomputed from the log-sum-exp.
 
 Calls enqueue on the current torch stream of the tensors' device and do not synchronise; outputs are new
 tensors.  A call that cannot be made raises (``ValueError`` for its arguments, ``RuntimeError`` for a
@@ -28,6 +30,9 @@ _SIGS = {
     "wubu_b200_resnorm_forward": (_ip, [ctypes.c_char_p, _vp]),
     "wubu_b200_resnorm_workspace": (_ll, [ctypes.c_char_p]),
     "wubu_b200_resnorm_backward": (_ip, [ctypes.c_char_p, _vp]),
+    "wubu_b200_attn_workspace": (_ll, [ctypes.c_char_p, _ip]),
+    "wubu_b200_attn_forward": (_ip, [ctypes.c_char_p, _vp]),
+    "wubu_b200_attn_backward": (_ip, [ctypes.c_char_p, _vp]),
 }
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTS = {"identity": 0, "lrelu": 1, "gelu": 2, "silu": 3}
@@ -289,3 +294,124 @@ def resnorm_backward(dr, dh, x, f, *, norm="layer", weight=None, bias=None, post
         _check(h.wubu_b200_resnorm_backward(pack(ws.data_ptr(), n), _stream(dev)), what)
     return {"dx": dx, "df": df, "dgate": dgate, "dweight": dweight, "dbias": dbias, "dpost_weight": dpost_weight,
             "dpost_bias": dpost_bias}
+
+
+# ---- attention --------------------------------------------------------------------------------------
+
+_ATTN = struct.Struct("@9if2P" + "P3q" * 4 + "P" + "P3q" * 4 + "Pq")
+_NO_VIEW = (0, 0, 0, 0)
+
+
+def _view(t):
+    """(t, (address, batch, token, head strides)): t itself where the library can address it (contiguous
+    last dimension, 16-byte aligned rows), else a copy."""
+    sb, st, sh, sd = t.stride()
+    B, T, H, D = t.shape
+    if (sd != 1 or t.data_ptr() & 15 or (B > 1 and (sb % 8 or sb < D)) or (T > 1 and (st % 8 or st < D))
+            or (H > 1 and (sh % 8 or sh < D))):
+        t = t.contiguous()
+        if t.data_ptr() & 15:
+            t = t.clone()
+        sb, st, sh, _ = t.stride()
+    return t, (t.data_ptr(), sb, st, sh)
+
+
+def _lens(n, B, dev, what):
+    if n is None:
+        return None
+    if n.shape != (B,) or n.device != dev:
+        raise ValueError(f"{what}: lengths are [{B}] on {dev}, got {tuple(n.shape)} on {n.device}")
+    if n.dtype != torch.int32 or not n.is_contiguous():
+        n = n.to(torch.int32).contiguous()
+    return n
+
+
+def _attn_operands(what, q, k, v, causal, window, scale, q_lens, k_lens):
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
+        raise ValueError(f"{what}: q is [B, Tq, Hq, D], k and v are [B, Tk, Hkv, D]")
+    B, Tq, Hq, D = q.shape
+    Bk, Tk, Hkv, Dk = k.shape
+    if B != Bk or D != Dk or (Hq % Hkv if Hkv else Hq):
+        raise ValueError(f"{what}: q {tuple(q.shape)} does not go with k {tuple(k.shape)}")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError(f"{what}: D is a multiple of 8 from 8 to 128, got {D}")
+    d = _DTYPES.get(q.dtype)
+    if d is None or d == 0 or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"{what}: bfloat16 or float16 tensors of one type")
+    if window < 0 or (scale is not None and not 0.0 < scale < float("inf")):
+        raise ValueError(f"{what}: window is not negative, scale is positive")
+    dev = _cuda(what, q, k, v)
+    ql, kl = _lens(q_lens, B, dev, what), _lens(k_lens, B, dev, what)
+    head = (d, B, Hq, Hkv, Tq, Tk, D, int(bool(causal)), min(int(window), 2 ** 30), scale or 0.0)
+    return dev, head, (_ptr(ql), _ptr(kl)), (ql, kl)
+
+
+def attention_forward(q, k, v, *, causal=False, window=0, scale=None, q_lens=None, k_lens=None):
+    """``(out, lse)``: softmax(scale q k^T) v over the visible keys, and the float32 log-sum-exp [B, Hq, Tq].
+
+    q ``[B, Tq, Hq, D]``, k and v ``[B, Tk, Hkv, D]`` (Hq a multiple of Hkv: query head h reads key head
+    h * Hkv // Hq); ``scale`` defaults to 1 / sqrt(D).  ``q_lens`` / ``k_lens``: int32 ``[B]`` on the device,
+    the lengths of padded items (what lies beyond may hold anything).  Query i sits at place
+    p = i + k_len - q_len among the keys and sees key j if j < k_len, j <= p (``causal``) and
+    |p - j| < window (``window`` > 0).  A query that sees nothing, or lies beyond q_len, has out 0 and lse -inf."""
+    what = "attention_forward"
+    dev, head, lens, hold = _attn_operands(what, q, k, v, causal, window, scale, q_lens, k_lens)
+    q, vq = _view(q)
+    k, vk = _view(k)
+    v, vv = _view(v)
+    B, Tq, Hq, D = q.shape
+    out = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=dev)
+    lse = torch.empty((B, Hq, Tq), dtype=torch.float32, device=dev)
+    body = (*head, *lens, *vq, *vk, *vv, out.data_ptr(), Tq * Hq * D, Hq * D, D, lse.data_ptr(), *_NO_VIEW * 4)
+    h = L()
+    with _on(dev):
+        n = _check(h.wubu_b200_attn_workspace(_ATTN.pack(*body, 0, 0), 0), what)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        _check(h.wubu_b200_attn_forward(_ATTN.pack(*body, _ptr(ws), n), _stream(dev)), what)
+    return out, lse
+
+
+def attention_backward(dout, q, k, v, out, lse, *, causal=False, window=0, scale=None, q_lens=None, k_lens=None):
+    """``(dq, dk, dv)`` for the gradient ``dout`` of ``attention_forward``'s out; ``out`` and ``lse`` are what it
+    returned for the same arguments.  The gradients of shared heads are sums over the heads that share them."""
+    what = "attention_backward"
+    dev, head, lens, hold = _attn_operands(what, q, k, v, causal, window, scale, q_lens, k_lens)
+    B, Tq, Hq, D = q.shape
+    for t in (dout, out):
+        if t.shape != q.shape or t.dtype != q.dtype or t.device != dev:
+            raise ValueError(f"{what}: dout and out have q's shape, type and device")
+    if lse.shape != (B, Hq, Tq) or lse.dtype != torch.float32 or lse.device != dev:
+        raise ValueError(f"{what}: lse is float32 [B, Hq, Tq]")
+    lse = lse.contiguous()
+    (q, vq), (k, vk), (v, vv), (out, vo), (dout, vg) = map(_view, (q, k, v, out, dout))
+    Tk, Hkv = k.shape[1:3]
+    dq = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=dev)
+    dk = torch.empty((B, Tk, Hkv, D), dtype=q.dtype, device=dev)
+    dv = torch.empty((B, Tk, Hkv, D), dtype=q.dtype, device=dev)
+    sq, skv = (Tq * Hq * D, Hq * D, D), (Tk * Hkv * D, Hkv * D, D)
+    body = (*head, *lens, *vq, *vk, *vv, *vo, lse.data_ptr(), *vg, dq.data_ptr(), *sq, dk.data_ptr(), *skv,
+            dv.data_ptr(), *skv)
+    h = L()
+    with _on(dev):
+        n = _check(h.wubu_b200_attn_workspace(_ATTN.pack(*body, 0, 0), 1), what)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        _check(h.wubu_b200_attn_backward(_ATTN.pack(*body, ws.data_ptr(), n), _stream(dev)), what)
+    return dq, dk, dv
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, opts):
+        out, lse = attention_forward(q, k, v, **opts)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.opts = opts
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        return (*attention_backward(dout, *ctx.saved_tensors, **ctx.opts), None)
+
+
+def attention(q, k, v, **opts):
+    """``attention_forward``'s out, differentiable by torch's autograd."""
+    return _Attention.apply(q, k, v, opts)
