@@ -31,32 +31,6 @@ WB_DEV float dot4(const float* x, const float* y) {
   return warp_sum(x[0] * y[0] + x[1] * y[1] + x[2] * y[2] + x[3] * y[3]);
 }
 
-// Forward, a warp per query: one pass over its keys with a running maximum and sum.
-template <typename T>
-__global__ void __launch_bounds__(128) attn_forward_kernel(const AttnParams p) {
-  const WubuB200Attn& a = p.a;
-  const int lane = threadIdx.x & 31, i = blockIdx.x * 4 + threadIdx.x / 32, h = blockIdx.y, b = blockIdx.z;
-  if (i >= a.Tq) return;
-  const AttnItem it(a, b);
-  float q[4], o[4] = {}, k[4], v[4], m = -INFINITY, l = 0.f;
-  row4(at<T>(a.q, b, i, h), a.D, lane, q);
-  for (int j = it.key_lo(a, i); j < it.key_hi(a, i); ++j) {
-    row4(at<T>(a.k, b, j, h / p.group), a.D, lane, k);
-    row4(at<T>(a.v, b, j, h / p.group), a.D, lane, v);
-    const float s = dot4(q, k) * a.scale, m1 = fmaxf(m, s);
-    const float c = m == -INFINITY ? 0.f : expf(m - m1), w = expf(s - m1);
-    l = l * c + w;
-#pragma unroll
-    for (int d = 0; d < 4; ++d) o[d] = o[d] * c + w * v[d];
-    m = m1;
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-  for (int d = 0; d < 4; ++d) o[d] *= inv;
-  put4(at<T>(a.out, b, i, h), a.D, lane, o);
-  if (lane == 0) a.lse[((long long)b * a.Hq + h) * a.Tq + i] = l > 0.f ? m + logf(l) : -INFINITY;
-}
-
 // delta = rowsum(dO * O) and the log-sum-exp in units of log 2, padded with what gives probability 0
 template <typename T>
 __global__ void __launch_bounds__(128) attn_delta_kernel(const AttnParams p) {
@@ -135,13 +109,12 @@ __global__ void __launch_bounds__(128) attn_dkv_kernel(const AttnParams p) {
 
 }  // namespace
 
-int attn_forward(const AttnParams& p, cudaStream_t st) {
-  const WubuB200Attn& a = p.a;
-  with_dtype(a.dtype, [&](auto t) {
-    typedef decltype(t) T;
-    attn_forward_kernel<T><<<dim3((a.Tq + 3) / 4, a.Hq, a.B), 128, 0, st>>>(p);
-  });
-  return ops_launched("attn_forward");
+bool attn_map(CUtensorMap* m, const WubuB200View& v, int B, int T, int H, int D) {
+  const uint64_t dims[4] = {(uint64_t)D, (uint64_t)T, (uint64_t)H, (uint64_t)B};
+  // the stride of a unit extent is never applied, but has to be a positive multiple of 16
+  const uint64_t strides[3] = {v.token ? (uint64_t)v.token * 2 : 16, v.head ? (uint64_t)v.head * 2 : 16,
+                               v.batch ? (uint64_t)v.batch * 2 : 16};
+  return make_map_16bit_4d(m, v.data, dims, strides, 64, kTile);
 }
 
 int attn_backward(const AttnParams& p, cudaStream_t st) {
@@ -213,7 +186,7 @@ extern "C" {
 long long wubu_b200_attn_workspace(const WubuB200Attn* a, int backward) {
   const int rc = check_shape(a);
   if (rc != WUBU_B200_OK) return rc == 1 ? 0 : rc;
-  return backward ? backward_bytes(*a) : 0;
+  return backward ? backward_bytes(*a) : attn_fwd_bytes(*a);
 }
 
 int wubu_b200_attn_forward(const WubuB200Attn* in, void* stream) {
@@ -221,6 +194,10 @@ int wubu_b200_attn_forward(const WubuB200Attn* in, void* stream) {
   const int rc = prepare(in, p);
   if (rc != WUBU_B200_OK) return rc == 1 ? WUBU_B200_OK : rc;
   if (p.a.Tq == 0) return WUBU_B200_OK;
+  if (const long long n = attn_fwd_bytes(p.a)) {
+    if (!p.a.workspace || !aligned16(p.a.workspace)) return WUBU_B200_ERR_ARG;
+    if (p.a.workspace_bytes < n) return WUBU_B200_ERR_NOMEM;
+  }
   p.err = ops_status_word();
   if (!p.err) return WUBU_B200_ERR_CUDA;
   return attn_forward(p, (cudaStream_t)stream);

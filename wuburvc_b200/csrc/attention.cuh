@@ -10,6 +10,9 @@ struct AttnParams {
   float* delta;      // backward: [B][Hq][t_pad] rowsum(dO * O)
   float* lse2;       // backward: [B][Hq][t_pad] lse in units of log 2; +infinity where a query sees nothing
   int t_pad;
+  int splits;        // forward: parts that the keys are split into, each with an out and an lse of its own
+  float* part;       // [splits][B][Hq][Tq][D]
+  float* part_lse;   // [splits][B][Hq][Tq]
   int* err;
   unsigned long long wait_ns;
 };
@@ -48,6 +51,97 @@ WB_DEV T* at(const WubuB200View& v, int b, int t, int h) {
 }
 
 int attn_forward(const AttnParams& p, cudaStream_t st);
+long long attn_fwd_bytes(const WubuB200Attn& a);  // the forward's workspace
 int attn_backward(const AttnParams& p, cudaStream_t st);
+
+// ---- tensor-core tiles ---------------------------------------------------------------------------
+// A tile is 128 tokens of one head in shared memory, as one box of 64 values a row (DP = 64) or two
+// (DP = 128), 16 KB each with 128-byte swizzle; columns from D on and tokens from T on are filled with zeros by
+// the copy.  The same tile serves as an operand along its values (K-major: q k^T, dO V^T) and along its
+// tokens (MN-major: P V, P^T dO, dS K, dS^T Q).
+constexpr int kTile = 128;
+constexpr uint32_t kBox = 128 * 128;  // bytes
+
+// The map of a view's tokens x values; false (with a message) if it cannot be encoded.
+bool attn_map(CUtensorMap* m, const WubuB200View& v, int B, int T, int H, int D);
+
+WB_DEV void load_tile(uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int t0, int h, int b, int boxes) {
+  for (int i = 0; i < boxes; ++i) tma_load_4d_warp(dst + i * kBox, m, bar, i * 64, t0, h, b);
+}
+WB_DEV uint64_t desc_k(const uint8_t* tile) { return make_sdesc(smem_u32(tile), 16, 1024, 2); }
+WB_DEV uint64_t desc_mn(const uint8_t* tile) { return make_sdesc(smem_u32(tile), kBox, 1024, 2); }
+
+// D[tmem] (+)= A B^T over the values of two tiles, both K-major; `ksteps` of 16
+WB_DEV void mma_values(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int ksteps) {
+  for (int k = 0; k < ksteps; ++k) {
+    const uint32_t o = ((k >> 2) * kBox + (k & 3) * 32u) >> 4;  // 4 steps of 32 bytes in a box's row
+    umma_f16_warp(d, a + o, b + o, idesc, k != 0);
+  }
+}
+// tcgen05.mma with A in tensor memory (128 rows, two 16-bit values a column)
+WB_DEV void umma_f16_ts_warp(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+WB_DEV void tmem_ld32_async(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+WB_DEV void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+WB_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+WB_DEV void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+WB_DEV void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+WB_DEV void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// A warp writes zeros over the tokens [from, 128) of a tile (what lies beyond an item's length may be
+// anything, and 0 x NaN is NaN), visibly to the tensor core.
+WB_DEV void zero_rows(uint8_t* tile, int from, int boxes) {
+  const int lane = threadIdx.x & 31;
+  for (int i = 0; i < boxes; ++i)
+    for (int o = from * 128 + lane * 16; o < (int)kBox; o += 512)
+      *reinterpret_cast<uint4*>(tile + i * kBox + o) = make_uint4(0, 0, 0, 0);
+  fence_async_smem();
+  __syncwarp();
+}
+
+// Moves registers between the warpgroups of a CTA (executed by whole warpgroups); the shares must add up
+// to no more than what the CTA was launched with.
+template <int N>
+WB_DEV void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+WB_DEV void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+WB_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 }  // namespace wb

@@ -72,6 +72,22 @@ bool make_map_bf16_3d(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1
   return true;
 }
 
+bool make_map_16bit_4d(CUtensorMap* m, const void* base, const uint64_t dims[4], const uint64_t strides_bytes[3],
+                       uint32_t b0, uint32_t b1) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
+  const cuuint64_t s[3] = {strides_bytes[0], strides_bytes[1], strides_bytes[2]};
+  const cuuint32_t box[4] = {b0, b1, 1, 1}, es[4] = {1, 1, 1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, s, box, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    fprintf(stderr, "wuburvc_b200: cuTensorMapEncodeTiled failed (%d) dims %llu %llu %llu %llu\n", (int)r,
+            (unsigned long long)d[0], (unsigned long long)d[1], (unsigned long long)d[2], (unsigned long long)d[3]);
+  return r == CUDA_SUCCESS;
+}
+
 // choose K chunk / stages for the forward-type kernel: about three stages, each holding as many
 // (tap, chunk) steps as fit (every stage costs the MMA warp one barrier round trip)
 static void pick_fwd_tiling(int c_in, int n_tile, int split, int& kc, int& stages, int& kgroup, size_t& smem) {

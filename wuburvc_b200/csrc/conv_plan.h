@@ -22,6 +22,11 @@ cudaError_t launch_tc_wgrad(const TcWgMaps& maps, const TcWgParams& p, dim3 grid
 bool make_map_bf16_3d(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uint64_t d2,
                       uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t b0, uint32_t b1, uint32_t b2);
 
+// Encodes a 4-D map of 16-bit elements with 128-byte swizzle: dims (d0 inner), byte strides of d1, d2, d3,
+// box (b0, b1, 1, 1) with b0 = 64.  Elements outside are filled with zeros.
+bool make_map_16bit_4d(CUtensorMap* m, const void* base, const uint64_t dims[4], const uint64_t strides_bytes[3],
+                       uint32_t b0, uint32_t b1);
+
 struct ConvLaunch {
   TcMaps maps;
   TcConvParams p;

@@ -1,6 +1,7 @@
 // ops.cuh — what the transformer training operators (act8.cu, resnorm.cu, attention*.cu) share: element
 // types, 16-byte loads and stores as floats, and the host-side checks.
 #pragma once
+#include <atomic>
 #include <cstdio>
 
 #include "../../include/wuburvc_b200.h"
@@ -10,6 +11,16 @@ namespace wb {
 
 // The operators' device status word (one per device, see wubu_b200_ops_sync); nullptr on a CUDA error.
 int* ops_status_word();
+
+// Raises a kernel's dynamic shared-memory limit, once per device (`devices`: the ones done).
+inline bool ops_smem_limit(const void* kernel, int bytes, std::atomic<uint64_t>& devices) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  if (devices.load() >> dev & 1) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  devices.fetch_or(uint64_t(1) << dev);
+  return true;
+}
 
 inline int ops_launched(const char* what) {
   const cudaError_t e = cudaGetLastError();
