@@ -9,6 +9,7 @@ struct AttnParams {
   int group;         // query heads to a key / value head
   float* delta;      // backward: [B][Hq][t_pad] rowsum(dO * O)
   float* lse2;       // backward: [B][Hq][t_pad] lse in units of log 2; +infinity where a query sees nothing
+  unsigned* norm_bits;  // backward, fp16: [2][B][Hkv] bits of the largest squared row norms of dO and of V
   int t_pad;
   int splits;        // forward: parts that the keys are split into, each with an out and an lse of its own
   float* part;       // [splits][B][Hq][Tq][D]
@@ -52,6 +53,7 @@ WB_DEV T* at(const WubuB200View& v, int b, int t, int h) {
 
 int attn_forward(const AttnParams& p, cudaStream_t st);
 long long attn_fwd_bytes(const WubuB200Attn& a);  // the forward's workspace
+long long attn_bwd_bytes(const WubuB200Attn& a);  // the backward's
 int attn_backward(const AttnParams& p, cudaStream_t st);
 
 // ---- tensor-core tiles ---------------------------------------------------------------------------
@@ -103,6 +105,21 @@ WB_DEV void tmem_ld32_async(uint32_t taddr, float* v) {
       : "r"(taddr));
 }
 WB_DEV void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// After tmem_wait_ld: ties 32 loaded values to this point, so that no use of them is moved above the wait.
+WB_DEV void tmem_use32(float* v) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile("" : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]),
+                 "+f"(v[i + 6]), "+f"(v[i + 7]));
+}
+template <int N>
+WB_DEV void tmem_load(uint32_t taddr, float* v) {  // N columns, a multiple of 32
+#pragma unroll
+  for (int g = 0; g < N; g += 32) tmem_ld32_async(taddr + g, v + g);
+  tmem_wait_ld();
+#pragma unroll
+  for (int g = 0; g < N; g += 32) tmem_use32(v + g);
+}
 WB_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 WB_DEV void tmem_st32(uint32_t taddr, const uint32_t* r) {
   asm volatile(

@@ -204,9 +204,7 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
       if (!ok) continue;
       tc_fence_after();
       float x[128];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) tmem_ld32_async(S + 32 * g, x + 32 * g);
-      tmem_wait_ld();
+      tmem_load<128>(S, x);
       const int j0 = j * kTile;
       if (j0 < all_lo || j0 + kTile > all_hi) {
         const int r0 = lo - j0, r1 = hi - j0;
@@ -228,8 +226,7 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
 #pragma unroll
           for (int g = 0; g < DP / 32; ++g) {
             float o[32];
-            tmem_ld32_async(O + 32 * g, o);
-            tmem_wait_ld();
+            tmem_load<32>(O + 32 * g, o);
 #pragma unroll
             for (int k = 0; k < 32; ++k) o[k] *= f;
             tmem_st32(O + 32 * g, reinterpret_cast<const uint32_t*>(o));
@@ -267,10 +264,7 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
 #pragma unroll
     for (int g = 0; g < DP / 32; ++g) {
       float o[32];
-      if (st1 > st0) {
-        tmem_ld32_async(O + 32 * g, o);
-        tmem_wait_ld();
-      }
+      if (st1 > st0) tmem_load<32>(O + 32 * g, o);
 #pragma unroll
       for (int k = 0; k < 32; ++k) o[k] = live ? o[k] * inv : bad ? l : 0.f;
       if (i >= a.Tq) continue;

@@ -17,6 +17,11 @@ int* ops_status_word() {
   static int* at[kMaxDevices];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return nullptr;
+  // a thread that has made no CUDA call yet (an autograd worker) has no current context, which the
+  // driver's tensor-map encoding needs
+  static thread_local bool in_context = false;
+  if (!in_context && cudaSetDevice(dev) != cudaSuccess) return nullptr;
+  in_context = true;
   std::lock_guard<std::mutex> lk(mu);
   if (!at[dev]) {
     void* p = nullptr;
