@@ -30,23 +30,51 @@ struct Act8 {
   int cols, nblk;
 };
 
+WB_DEV float exp2f_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Phi(x) and the density phi(x) of the normal distribution from one exponential and one reciprocal:
+// Phi(-|x|) is e^(-x^2/2) times a polynomial in t = 1 / (1 + p |x| / sqrt 2) (Abramowitz and Stegun,
+// Handbook of Mathematical Functions, 7.1.26; absolute error below 1e-7).  Straight-line code: a
+// library erff in two ranges, with expf beside it, made the backward twice as slow as its memory traffic.
+WB_DEV void normal(float x, float& cdf, float& density) {
+  const float z = fabsf(x);
+  const float t = __fdividef(1.f, fmaf(0.3275911f * 0.70710678118654752f, z, 1.f));
+  const float e = exp2f_fast(x * x * -0.72134752044448170f);  // e^(-x^2/2)
+  float s = fmaf(1.061405429f, t, -1.453152027f);
+  s = fmaf(s, t, 1.421413741f);
+  s = fmaf(s, t, -0.284496736f);
+  s = fmaf(s, t, 0.254829592f);
+  const float tail = 0.5f * s * t * e;
+  cdf = x > 0.f ? 1.f - tail : tail;
+  density = e * 0.39894228040143268f;
+}
+
 WB_DEV float act_value(float x, int act, float slope) {
   if (act == WUBU_B200_ACT_LRELU) return x > 0.f ? x : slope * x;
-  if (act == WUBU_B200_ACT_GELU) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
-  if (act == WUBU_B200_ACT_SILU) return x / (1.f + expf(-x));
+  if (act == WUBU_B200_ACT_GELU) {
+    float cdf, density;
+    normal(x, cdf, density);
+    return x * cdf;
+  }
+  if (act == WUBU_B200_ACT_SILU) return __fdividef(x, 1.f + __expf(-x));
   return x;
 }
-// act(x) and act'(x), sharing the error function or the sigmoid
+// act(x) and act'(x)
 WB_DEV void act_both(float x, int act, float slope, float& y, float& d) {
   if (act == WUBU_B200_ACT_LRELU) {
     d = x > 0.f ? 1.f : slope;
     y = x * d;
   } else if (act == WUBU_B200_ACT_GELU) {
-    const float phi = 0.5f * (1.f + erff(x * 0.70710678118654752f));
-    y = x * phi;
-    d = phi + x * (expf(-0.5f * x * x) * 0.39894228040143268f);
+    float cdf, density;
+    normal(x, cdf, density);
+    y = x * cdf;
+    d = fmaf(x, density, cdf);
   } else if (act == WUBU_B200_ACT_SILU) {
-    const float t = 1.f / (1.f + expf(-x));
+    const float t = __fdividef(1.f, 1.f + __expf(-x));
     y = x * t;
     d = t * (1.f + x * (1.f - t));
   } else {

@@ -73,22 +73,52 @@ WB_DEV void load_tile(uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int t0,
 WB_DEV uint64_t desc_k(const uint8_t* tile) { return make_sdesc(smem_u32(tile), 16, 1024, 2); }
 WB_DEV uint64_t desc_mn(const uint8_t* tile) { return make_sdesc(smem_u32(tile), kBox, 1024, 2); }
 
-// D[tmem] (+)= A B^T over the values of two tiles, both K-major; `ksteps` of 16
-WB_DEV void mma_values(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int ksteps) {
-  for (int k = 0; k < ksteps; ++k) {
-    const uint32_t o = ((k >> 2) * kBox + (k & 3) * 32u) >> 4;  // 4 steps of 32 bytes in a box's row
-    umma_f16_warp(d, a + o, b + o, idesc, k != 0);
-  }
-}
-// tcgen05.mma with A in tensor memory (128 rows, two 16-bit values a column)
-WB_DEV void umma_f16_ts_warp(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// Four steps of 16 in one go (one election, the later steps' operands by constant offsets): D[tmem] (+)= A B^T
+// with both operands in shared memory along their rows.
+WB_DEV void mma4_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
       "elect.sync _|e, 0xffffffff;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "add.u64 a1, %1, 2;\n\tadd.u64 b1, %2, 2;\n\t"
+      "add.u64 a2, %1, 4;\n\tadd.u64 b2, %2, 4;\n\t"
+      "add.u64 a3, %1, 6;\n\tadd.u64 b3, %2, 6;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, 1;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, 1;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, 1;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+// The same with A in tensor memory (128 rows, two 16-bit values a column) and B along its tokens (16 tokens
+// are 2 KB).
+WB_DEV void mma4_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 b1, b2, b3;\n\t.reg .b32 a1, a2, a3;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "add.u32 a1, %1, 8;\n\tadd.u64 b1, %2, 128;\n\t"
+      "add.u32 a2, %1, 16;\n\tadd.u64 b2, %2, 256;\n\t"
+      "add.u32 a3, %1, 24;\n\tadd.u64 b3, %2, 384;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, 1;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, 1;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, 1;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D[tmem] = A B^T over the values of two tiles; `ksteps` (at most DP / 16) steps of 16
+template <int DP>
+WB_DEV void mma_values(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int ksteps) {
+#pragma unroll
+  for (int box = 0; box < DP / 64; ++box) {
+    const uint64_t ab = a + box * (kBox >> 4), bb = b + box * (kBox >> 4);
+    if (ksteps >= 4 * box + 4) {
+      mma4_ss(d, ab, bb, idesc, box);
+    } else {
+      for (int k = 4 * box; k < ksteps; ++k) umma_f16_warp(d, ab + 2 * (k & 3), bb + 2 * (k & 3), idesc, k != 0);
+    }
+  }
 }
 
 WB_DEV void tmem_ld32_async(uint32_t taddr, float* v) {
@@ -135,6 +165,19 @@ WB_DEV void tmem_st32(uint32_t taddr, const uint32_t* r) {
 WB_DEV void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// mbar_wait_warp with a first test in line: most waits of the pipeline are for phases that are long complete.
+WB_DEV bool bar_wait(uint64_t* bar, uint32_t parity, int* err, int code, unsigned long long limit_ns) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  if (__all_sync(0xffffffffu, done)) return true;
+  return mbar_wait_warp(bar, parity, err, code, limit_ns);
+}
 WB_DEV void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // A warp writes zeros over the tokens [from, 128) of a tile (what lies beyond an item's length may be
@@ -154,6 +197,34 @@ template <int N>
 WB_DEV void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 WB_DEV void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Two float32 operations in one instruction.
+WB_DEV uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+WB_DEV void each(uint64_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+WB_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+WB_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+WB_DEV uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+WB_DEV float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 WB_DEV float ex2(float x) {
   float y;

@@ -67,9 +67,6 @@ WB_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar)
       : "memory");
 }
 
-// the 16-row steps of an A operand that two warpgroups wrote as 2 x 32 columns, 64 apart
-WB_DEV uint32_t half_col(int k) { return (uint32_t)((k >> 2) * 64 + (k & 3) * 8); }
-
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_constant__ AttnParams p, int kv_ctas) {
@@ -164,7 +161,7 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
       int t = t0, h = kv ? hq : hk;
       for (int n = 0; n < steps; ++n) {
         const int sa = slot_a(n), sb = slot_b(n);
-        if (ok && n >= na) ok = mbar_wait_warp(&bar.a_empty[sa], phase_a(n) ^ 1u, p.err, ERR_WAIT_EMPTY, p.wait_ns);
+        if (ok && n >= na) ok = bar_wait(&bar.a_empty[sa], phase_a(n) ^ 1u, p.err, ERR_WAIT_EMPTY, p.wait_ns);
         if (ok) {
           fa.fill(sa, phase_a(n));
           mbar_expect_tx_warp(&bar.a_full[sa], kTileBytes + (kv ? 2 * kTile * 4 : 0));
@@ -175,7 +172,7 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
             bulk_load(rows + sa * 2 * kTile + kTile, p.delta + r, kTile * 4, &bar.a_full[sa]);
           }
         }
-        if (ok && n >= kStagesB) ok = mbar_wait_warp(&bar.b_empty[sb], phase_b(n) ^ 1u, p.err, ERR_WAIT_EMPTY, p.wait_ns);
+        if (ok && n >= kStagesB) ok = bar_wait(&bar.b_empty[sb], phase_b(n) ^ 1u, p.err, ERR_WAIT_EMPTY, p.wait_ns);
         if (ok) {
           fb.fill(sb, phase_b(n));
           mbar_expect_tx_warp(&bar.b_full[sb], kTileBytes);
@@ -194,40 +191,40 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
       const uint32_t id_o = make_idesc(128, (a.D + 15) / 16 * 16, 0, 1, kBf16);
       const int ksteps = (a.D + 15) / 16;
       const uint64_t dr0 = desc_k(res0), dr1 = desc_k(res1);
-      bool ok = steps > 0 ? mbar_wait_warp(&bar.res_full, 0, p.err, ERR_WAIT_FULL, p.wait_ns) : true;
+      bool ok = steps > 0 ? bar_wait(&bar.res_full, 0, p.err, ERR_WAIT_FULL, p.wait_ns) : true;
       // rows of step n's tiles beyond the item's length
       auto valid = [&](int n) { return (kv ? it.ql : it.kl) - (t0 + n % per_head) * kTile; };
       auto wait_a = [&](int n) {
         const int st = slot_a(n);
-        if (ok) ok = mbar_wait_warp(&bar.a_full[st], phase_a(n), p.err, ERR_WAIT_FULL, p.wait_ns);
+        if (ok) ok = bar_wait(&bar.a_full[st], phase_a(n), p.err, ERR_WAIT_FULL, p.wait_ns);
         if (ok && valid(n) < kTile) zero_rows(ra + st * kTileBytes, max(valid(n), 0), kBoxes);
       };
       auto wait_b = [&](int n) {
         const int st = slot_b(n);
-        if (ok) ok = mbar_wait_warp(&bar.b_full[st], phase_b(n), p.err, ERR_WAIT_FULL, p.wait_ns);
+        if (ok) ok = bar_wait(&bar.b_full[st], phase_b(n), p.err, ERR_WAIT_FULL, p.wait_ns);
         if (ok && valid(n) < kTile) zero_rows(rb + st * kTileBytes, max(valid(n), 0), kBoxes);
       };
       auto issue_s = [&](int n) {
         wait_a(n);
         const int buf = kv ? 0 : n & 1;
         if (ok) {
-          mma_values(tmem + 128 * buf, dr0, desc_k(ra + slot_a(n) * kTileBytes), id_s, ksteps);
+          mma_values<DP>(tmem + 128 * buf, dr0, desc_k(ra + slot_a(n) * kTileBytes), id_s, ksteps);
           umma_commit_warp(&bar.s_full[buf]);
         }
       };
       auto issue_dp = [&](int n) {
         wait_b(n);
         if (ok) {
-          mma_values(tDP, dr1, desc_k(rb + slot_b(n) * kTileBytes), id_s, ksteps);
+          mma_values<DP>(tDP, dr1, desc_k(rb + slot_b(n) * kTileBytes), id_s, ksteps);
           umma_commit_warp(&bar.dp_full);
           if (!kv) umma_commit_warp(&bar.b_empty[slot_b(n)]);  // nothing else reads V
         }
       };
-      // acc += (A in tensor memory, 128 x 128) x tile
+      // acc += (A in tensor memory, 128 x 128, its halves 64 columns apart) x tile
       auto issue_acc = [&](uint32_t acc, uint32_t src, const uint8_t* tile_, int n) {
         const uint64_t d = desc_mn(tile_);
-        for (int k = 0; k < kTile / 16; ++k)
-          umma_f16_ts_warp(acc, src + half_col(k), d + k * (2048u >> 4), id_o, (n > 0) | (k != 0));
+        mma4_ts(acc, src, d, id_o, n > 0);
+        mma4_ts(acc, src + 64, d + (4 * 2048u >> 4), id_o, 1);
       };
       if (steps > 0) {
         issue_s(0);
@@ -237,12 +234,12 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
       for (int n = 0; n < steps; ++n) {
         const uint32_t ph = n & 1;
         if (kv) {
-          if (ok) ok = mbar_wait_warp(&bar.p_ready, ph, p.err, ERR_WAIT_ACC, p.wait_ns);
+          if (ok) ok = bar_wait(&bar.p_ready, ph, p.err, ERR_WAIT_ACC, p.wait_ns);
           tc_fence_after();
           if (ok) issue_acc(tAcc0, tmem, rb + slot_b(n) * kTileBytes, n);
           if (n + 1 < steps) issue_s(n + 1);
         }
-        if (ok) ok = mbar_wait_warp(&bar.ds_ready, ph, p.err, ERR_WAIT_ACC, p.wait_ns);
+        if (ok) ok = bar_wait(&bar.ds_ready, ph, p.err, ERR_WAIT_ACC, p.wait_ns);
         tc_fence_after();
         if (ok) {
           issue_acc(tAcc1, tDP, ra + slot_a(n) * kTileBytes, n);
@@ -255,7 +252,7 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
       if (ok) umma_commit_warp(&bar.acc_full);
       // every MMA this warp issued has completed before TMEM is released (also after a timed-out wait)
       umma_commit_warp(&bar.mma_done);
-      mbar_wait_warp(&bar.mma_done, 0, p.err, ERR_WAIT_ACC, p.wait_ns);
+      bar_wait(&bar.mma_done, 0, p.err, ERR_WAIT_ACC, p.wait_ns);
     }
   } else {
     regs_inc<216>();
@@ -280,10 +277,10 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
     for (int n = 0; n < steps; ++n) {
       const int st = slot_a(n), col0 = (t0 + n % per_head) * kTile + 64 * half;
       const uint32_t S = tmem + (kv ? 0 : 128 * (n & 1)) + lanes + 64 * half;
-      if (kv && ok) ok = mbar_wait_warp(&bar.a_full[st], phase_a(n), p.err, ERR_WAIT_FULL, p.wait_ns);
+      if (kv && ok) ok = bar_wait(&bar.a_full[st], phase_a(n), p.err, ERR_WAIT_FULL, p.wait_ns);
       if (ok)
-        ok = kv ? mbar_wait_warp(&bar.s_full[0], n & 1, p.err, ERR_WAIT_ACC, p.wait_ns)
-                : mbar_wait_warp(&bar.s_full[n & 1], (n >> 1) & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
+        ok = kv ? bar_wait(&bar.s_full[0], n & 1, p.err, ERR_WAIT_ACC, p.wait_ns)
+                : bar_wait(&bar.s_full[n & 1], (n >> 1) & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
       if (!ok) continue;
       tc_fence_after();
       float x[64];
@@ -317,7 +314,7 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.p_ready);
       }
-      ok = mbar_wait_warp(&bar.dp_full, n & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
+      ok = bar_wait(&bar.dp_full, n & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
       if (!ok) continue;
       tc_fence_after();
       float y[64];
@@ -342,7 +339,7 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.ds_ready);
     }
-    if (steps > 0 && ok) ok = mbar_wait_warp(&bar.acc_full, 0, p.err, ERR_WAIT_ACC, p.wait_ns);
+    if (steps > 0 && ok) ok = bar_wait(&bar.acc_full, 0, p.err, ERR_WAIT_ACC, p.wait_ns);
     tc_fence_after();
     // the accumulators, half of the columns to each warpgroup
     const bool live = hi > lo && steps > 0 && ok;

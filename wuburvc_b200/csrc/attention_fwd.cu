@@ -9,9 +9,11 @@
 //
 // A CTA owns two query tiles of 128 rows of one head (two streams).  Per stream the scores S (128 x 128
 // fp32) and the output accumulator live in tensor memory; four warps read S, one row a thread, and
-// write P over it, from where the second product reads it.  While the warps of one stream work on
-// their exponentials, the tensor core runs the other stream's products.  K and V tiles arrive by TMA
-// in rings of two and serve both streams.
+// write P back in two halves, from where the second product reads it as its A operand; a warp of its
+// own issues the stream's products.  While the warps of one stream work on their exponentials, the
+// tensor core runs the other stream's products.  K and V tiles arrive by TMA in rings and serve both.
+// Up to 64 values a row, tensor memory has room for P beside S: the next scores are then issued as soon
+// as S has been read and the streams never wait for a product.  At 128 values P lies over S.
 #include <type_traits>
 
 #include "attention.cuh"
@@ -19,11 +21,10 @@
 namespace wb {
 namespace {
 
-constexpr int kStages = 2;
 // Eight softmax warps (a row of 128 scores in registers each thread), and a warpgroup of which one warp
 // loads and one issues the products.  384 threads are launched with 168 registers; the split 256 x 216 +
 // 128 x 72 is the same 64512.
-constexpr int kProducer = 8, kMma = 9, kThreads = 384;
+constexpr int kProducer = 8, kMma = 9, kThreads = 384;  // kMma + s issues stream s
 
 struct AttnFwdMaps {
   CUtensorMap q, k, v;
@@ -38,19 +39,25 @@ struct FwdShift<f16> {
   static constexpr float value = 6.f;
 };
 
+template <int DP>
+constexpr int kFwdStages = DP == 64 ? 3 : 2;  // tiles in each of the two rings
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_constant__ AttnParams p) {
   constexpr int kBoxes = DP / 64;
   constexpr uint32_t kTileBytes = kBoxes * kBox;
+  constexpr int kStages = kFwdStages<DP>;
   constexpr float kShift = FwdShift<T>::value;
+  constexpr bool kApart = DP == 64;  // P has columns of its own
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* qt = smem;
   uint8_t* kt = qt + 2 * kTileBytes;
   uint8_t* vt = kt + kStages * kTileBytes;
+  // per stream: S complete; S read (kApart); the halves of P written; the product that read P done
   __shared__ uint64_t q_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2],
-      p_ready[2], o_full[2], mma_done;
+      s_read[2], p_ready[2][2], pv_done[2], mma_done[2];
   __shared__ uint32_t tmem_slot;
 
   const WubuB200Attn& a = p.a;
@@ -87,23 +94,27 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_ready[i], 4);
-      mbar_init(&o_full[i], 1);
+      mbar_init(&s_read[i], 4);
+      mbar_init(&p_ready[i][0], 4);
+      mbar_init(&p_ready[i][1], 4);
+      mbar_init(&pv_done[i], 1);
+      mbar_init(&mma_done[i], 1);
     }
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < kStages; ++i) {  // a tile is free once both streams are done with it
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], 2);
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_empty[i], 2);
     }
-    mbar_init(&mma_done, 1);
     fence_barrier_init();
   }
   if (warp == kMma) tmem_alloc(&tmem_slot, 512);
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 256 + DP};
+  // columns: S at 0 and 128; apart, P at 256 and 320 and O at 384 and 448; else P over S and O at 256 and 384
+  auto col_p = [&](int s) { return tmem + (kApart ? 256 + 64 * s : 128 * s); };
+  auto col_o = [&](int s) { return tmem + (kApart ? 384 + 64 * s : 256 + 128 * s); };
 
   if (warp >= kProducer) {
     regs_dec<72>();
@@ -121,13 +132,13 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
       for (int j = u0; j < u1; ++j) {
         const int n = j - u0, st = n % kStages;
         const uint32_t ph = (n / kStages) & 1;
-        if (ok && n >= kStages) ok = mbar_wait_warp(&k_empty[st], ph ^ 1u, p.err, ERR_WAIT_EMPTY, p.wait_ns);
+        if (ok && n >= kStages) ok = bar_wait(&k_empty[st], ph ^ 1u, p.err, ERR_WAIT_EMPTY, p.wait_ns);
         if (ok) {
           fk.fill(st, ph);
           mbar_expect_tx_warp(&k_full[st], kTileBytes);
           load_tile(kt + st * kTileBytes, &maps.k, &k_full[st], j * kTile, hk, b, kBoxes);
         }
-        if (ok && n >= kStages) ok = mbar_wait_warp(&v_empty[st], ph ^ 1u, p.err, ERR_WAIT_EMPTY, p.wait_ns);
+        if (ok && n >= kStages) ok = bar_wait(&v_empty[st], ph ^ 1u, p.err, ERR_WAIT_EMPTY, p.wait_ns);
         if (ok) {
           fv.fill(st, ph);
           mbar_expect_tx_warp(&v_full[st], kTileBytes);
@@ -137,58 +148,72 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
       fq.drain(q_full, p.err, p.wait_ns);  // no copy of this CTA may land after it exits
       fk.drain(k_full, p.err, p.wait_ns);
       fv.drain(v_full, p.err, p.wait_ns);
-    } else if (warp == kMma) {
+    } else if (warp < kMma + 2) {
+      const int s = warp - kMma;
+      const int st0 = s ? t0[1] : t0[0], st1 = s ? t1[1] : t1[0];
       constexpr int kBf16 = std::is_same<T, bf16>::value;
       const uint32_t id_s = make_idesc(128, 128, 0, 0, kBf16);
       const uint32_t id_o = make_idesc(128, (a.D + 15) / 16 * 16, 0, 1, kBf16);
       const int ksteps = (a.D + 15) / 16;
+      const uint64_t dq = desc_k(qt + s * kTileBytes);
+      const uint32_t P = col_p(s), O = col_o(s), S = tmem + 128 * s;
       bool ok = true;
-      uint32_t pph[2] = {0, 0};
-      for (int j = u0 - 1; j < u1; ++j) {
-        const int n = j - u0, st = n % kStages;
-        const bool next = j + 1 < u1;
-        const int nst = (n + 1) % kStages;
-        uint8_t* vtile = vt + (n < 0 ? 0 : st) * kTileBytes;
-        if (n >= 0) {
-          if (ok) ok = mbar_wait_warp(&v_full[st], (n / kStages) & 1, p.err, ERR_WAIT_FULL, p.wait_ns);
-          const int valid = it.kl - j * kTile;
-          if (ok && valid < kTile) zero_rows(vtile, max(valid, 0), kBoxes);
+      uint32_t ph = 0;
+      // the scores against key tile j, or a pass by a tile that the stream does not meet
+      auto issue_s = [&](int j) {
+        const int n = j - u0, sl = n % kStages;
+        if (ok) ok = bar_wait(&k_full[sl], (n / kStages) & 1, p.err, ERR_WAIT_FULL, p.wait_ns);
+        if (!ok) return;
+        if (j < st0 || j >= st1) {
+          if (lane == 0) mbar_arrive(&k_empty[sl]);
+          return;
         }
-        if (ok && next) ok = mbar_wait_warp(&k_full[nst], ((n + 1) / kStages) & 1, p.err, ERR_WAIT_FULL, p.wait_ns);
+        mma_values<DP>(S, dq, desc_k(kt + sl * kTileBytes), id_s, ksteps);
+        umma_commit_warp(&s_full[s]);
+        umma_commit_warp(&k_empty[sl]);
+      };
+      if (st1 > st0) ok = bar_wait(&q_full[s], 0, p.err, ERR_WAIT_FULL, p.wait_ns);
+      if (u0 < u1) issue_s(u0);
+      for (int j = u0; j < u1; ++j) {
+        const int n = j - u0, sl = n % kStages;
+        const bool mine = j >= st0 && j < st1;
+        if (kApart) {
+          if (mine && ok) ok = bar_wait(&s_read[s], ph, p.err, ERR_WAIT_ACC, p.wait_ns);
+          tc_fence_after();
+          if (j + 1 < u1) issue_s(j + 1);
+        }
+        if (ok) ok = bar_wait(&v_full[sl], (n / kStages) & 1, p.err, ERR_WAIT_FULL, p.wait_ns);
+        if (mine) {
+          uint8_t* tile = vt + sl * kTileBytes;
+          const int valid = it.kl - j * kTile;  // both streams may clear the same rows
+          if (ok && valid < kTile) zero_rows(tile, max(valid, 0), kBoxes);
+          const uint64_t dv = desc_mn(tile);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          if (n >= 0 && j >= t0[s] && j < t1[s]) {
-            if (ok) ok = mbar_wait_warp(&p_ready[s], pph[s], p.err, ERR_WAIT_ACC, p.wait_ns);
-            pph[s] ^= 1u;
+          for (int half = 0; half < 2; ++half) {
+            if (ok) ok = bar_wait(&p_ready[s][half], ph, p.err, ERR_WAIT_ACC, p.wait_ns);
             tc_fence_after();
-            if (ok) {
-              const uint64_t dv = desc_mn(vtile);
-              for (int k = 0; k < kTile / 16; ++k)
-                umma_f16_ts_warp(tO[s], tS[s] + k * 8, dv + k * (2048u >> 4), id_o, (j > t0[s]) | (k != 0));
-              if (j == t1[s] - 1) umma_commit_warp(&o_full[s]);
-            }
+            if (ok) mma4_ts(O, P + 32 * half, dv + half * (4 * 2048u >> 4), id_o, (j > st0) | half);
           }
-          if (next && j + 1 >= t0[s] && j + 1 < t1[s]) {
-            if (j + 1 == t0[s] && ok) ok = mbar_wait_warp(&q_full[s], 0, p.err, ERR_WAIT_FULL, p.wait_ns);
-            if (ok) {
-              mma_values(tS[s], desc_k(qt + s * kTileBytes), desc_k(kt + nst * kTileBytes), id_s, ksteps);
-              umma_commit_warp(&s_full[s]);
-            }
+          ph ^= 1u;
+          if (ok) {
+            umma_commit_warp(&pv_done[s]);
+            umma_commit_warp(&v_empty[sl]);
           }
+        } else if (ok && lane == 0) {
+          mbar_arrive(&v_empty[sl]);
         }
-        if (ok && n >= 0) umma_commit_warp(&v_empty[st]);
-        if (ok && next) umma_commit_warp(&k_empty[nst]);
+        if (!kApart && j + 1 < u1) issue_s(j + 1);
       }
       // every MMA this warp issued has completed before TMEM is released (also after a timed-out wait)
-      umma_commit_warp(&mma_done);
-      mbar_wait_warp(&mma_done, 0, p.err, ERR_WAIT_ACC, p.wait_ns);
+      umma_commit_warp(&mma_done[s]);
+      bar_wait(&mma_done[s], 0, p.err, ERR_WAIT_ACC, p.wait_ns);
     }
   } else {
     regs_inc<216>();
     const int s = warp >> 2;
     const int sq0 = s ? q0[1] : q0[0], st0 = s ? t0[1] : t0[0], st1 = s ? t1[1] : t1[0];
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t S = tmem + 128 * s + lanes, O = tmem + 256 + DP * s + lanes;
+    const uint32_t S = tmem + 128 * s + lanes, O = col_o(s) + lanes, P = col_p(s) + lanes;
     const int i = sq0 + (warp & 3) * 32 + lane;
     const int lo = it.key_lo(a, i), hi = it.key_hi(a, i);
     // key tiles that every live row of the query tile sees whole need no mask
@@ -199,12 +224,16 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
     bool ok = true;
     uint32_t ph = 0;
     for (int j = st0; j < st1; ++j) {
-      if (ok) ok = mbar_wait_warp(&s_full[s], ph, p.err, ERR_WAIT_ACC, p.wait_ns);
-      ph ^= 1u;
+      if (ok) ok = bar_wait(&s_full[s], ph, p.err, ERR_WAIT_ACC, p.wait_ns);
       if (!ok) continue;
       tc_fence_after();
       float x[128];
       tmem_load<128>(S, x);
+      if (kApart) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_read[s]);
+      }
       const int j0 = j * kTile;
       if (j0 < all_lo || j0 + kTile > all_hi) {
         const int r0 = lo - j0, r1 = hi - j0;
@@ -213,16 +242,23 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
       }
       float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-      for (int k = 4; k < 128; ++k) mx[k & 3] = fmaxf(mx[k & 3], x[k]);
-      const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      for (int k = 4; k < 124; k += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[k + e], x[k + 4 + e]);
+      const float mt = max3(max3(mx[0], mx[1], x[124]), max3(mx[2], mx[3], x[125]), fmaxf(x[126], x[127]));
       // move m when the maximum has outgrown it by 2^8 (or was not set)
       const bool move = mt > m && (m == -INFINITY || (mt - m) * c > 8.f);
-      if (__any_sync(0xffffffffu, move)) {
+      const bool any_move = __any_sync(0xffffffffu, move);
+      // apart, S may be ahead of the product that last read P and added to O; over S it cannot be
+      if (kApart && j > st0) ok = bar_wait(&pv_done[s], ph ^ 1u, p.err, ERR_WAIT_ACC, p.wait_ns);
+      ph ^= 1u;
+      if (!ok) continue;
+      if (any_move) {
         const float f = !move ? 1.f : m == -INFINITY ? 0.f : ex2((m - mt) * c);
         if (move) m = mt;
         l *= f;
         if (j > st0) {
-          // S of this tile is complete, and with it the product that last added to O
+          tc_fence_after();
 #pragma unroll
           for (int g = 0; g < DP / 32; ++g) {
             float o[32];
@@ -234,26 +270,32 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
         }
       }
       const float mc = (m == -INFINITY ? 0.f : m * c) - kShift;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t cc = two(c, c), mm = two(-mc, -mc);
+      uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
+        float* y = x + 64 * g;
         uint32_t w[32];
 #pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          const float e0 = ex2(fmaf(x[64 * g + 2 * k], c, -mc)), e1 = ex2(fmaf(x[64 * g + 2 * k + 1], c, -mc));
-          sum[(2 * k) & 3] += e0;
-          sum[(2 * k + 1) & 3] += e1;
-          w[k] = pack2(e0, e1, T());
-        }
-        tmem_st32(S + 32 * g, w);
+        for (int k = 0; k < 64; k += 2) each(fma2(two(y[k], y[k + 1]), cc, mm), y[k], y[k + 1]);
+#pragma unroll
+        for (int k = 0; k < 64; ++k) y[k] = ex2(y[k]);
+#pragma unroll
+        for (int k = 0; k < 64; k += 2) sum[k / 2 & 3] = add2(sum[k / 2 & 3], two(y[k], y[k + 1]));
+#pragma unroll
+        for (int k = 0; k < 32; ++k) w[k] = pack2(y[2 * k], y[2 * k + 1], T());
+        tmem_st32(P + 32 * g, w);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[s][g]);
       }
-      tmem_wait_st();
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[s]);
+      float l0, l1;
+      each(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), l0, l1);
+      l += l0 + l1;
     }
-    if (st1 > st0 && ok) ok = mbar_wait_warp(&o_full[s], 0, p.err, ERR_WAIT_ACC, p.wait_ns);
+    // the last product: its phase is that of the number of tiles before it
+    if (st1 > st0 && ok) ok = bar_wait(&pv_done[s], ph ^ 1u, p.err, ERR_WAIT_ACC, p.wait_ns);
     tc_fence_after();
     const bool live = l > 0.f && hi > lo && st1 > st0 && ok;
     const bool bad = hi > lo && st1 > st0 && !(l == l);  // a NaN among the scores stays visible
@@ -317,7 +359,7 @@ __global__ void __launch_bounds__(128) attn_fwd_join_kernel(const AttnParams p) 
 template <typename T, int DP>
 int launch_fwd(const AttnFwdMaps& maps, const AttnParams& p, cudaStream_t st) {
   const WubuB200Attn& a = p.a;
-  constexpr int smem = (2 + 2 * kStages) * (DP / 64) * (int)kBox + 1024;
+  constexpr int smem = (2 + 2 * kFwdStages<DP>) * (DP / 64) * (int)kBox + 1024;
   static std::atomic<uint64_t> devices{0};
   if (!ops_smem_limit((const void*)attn_fwd_tc_kernel<T, DP>, smem, devices)) return WUBU_B200_ERR_CUDA;
   const int npairs = (a.Tq + 2 * kTile - 1) / (2 * kTile);

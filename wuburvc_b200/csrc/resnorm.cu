@@ -7,15 +7,20 @@
 // The backward recomputes both norms from x and f, so that the forward keeps no statistics.
 //
 // A group of threads owns a row and holds it in registers, 8 values a thread, so each tensor is read
-// once and written once (bound by HBM).  In the backward a thread meets the same columns in every
-// row of its block's range and sums the parameter gradients in registers; the blocks' partial sums
-// are added in a fixed order by a second kernel.
+// once and written once (bound by HBM).  A block runs several groups, each with a barrier of its own, over
+// a range of one item's rows: the parameter vectors stay in registers, the next row is loaded before the
+// current one's sums are taken, and in the backward a thread meets the same columns in every row and
+// adds up the parameter gradients in registers; the blocks' partial sums are added in a fixed order by a
+// second kernel.
+#include <type_traits>
+
 #include "ops.cuh"
 
 namespace wb {
 namespace {
 
-constexpr int kMaxCols = 8192;  // 1024 threads x 8 values
+constexpr int kMaxCols = 8192;   // 1024 threads x 8 values
+constexpr int kThreads = 384;    // threads a block, where a row needs no more
 
 struct RowReduce {  // sums over a row's group of warps; four buffers in turn need one barrier a sum
   float2* buf;      // [4][rows][warps]
@@ -30,7 +35,7 @@ struct RowReduce {  // sums over a row's group of warps; four buffers in turn ne
     float2* mine = buf + (turn * rows + row) * warps;
     turn = (turn + 1) & 3;
     if (lane == 0) mine[warp] = make_float2(a, b);
-    __syncthreads();
+    asm volatile("bar.sync %0, %1;" ::"r"(row + 1), "r"(warps * 32) : "memory");
     a = b = 0.f;
     for (int i = 0; i < warps; ++i) {
       a += mine[i].x;
@@ -38,6 +43,24 @@ struct RowReduce {  // sums over a row's group of warps; four buffers in turn ne
     }
     return make_float2(a, b);
   }
+  WB_DEV float operator()(float a) {
+#pragma unroll
+    for (int m = 16; m; m >>= 1) a += __shfl_xor_sync(0xffffffffu, a, m);
+    if (warps == 1) return a;
+    float2* mine = buf + (turn * rows + row) * warps;
+    turn = (turn + 1) & 3;
+    if (lane == 0) mine[warp].x = a;
+    asm volatile("bar.sync %0, %1;" ::"r"(row + 1), "r"(warps * 32) : "memory");
+    a = 0.f;
+    for (int i = 0; i < warps; ++i) a += mine[i].x;
+    return a;
+  }
+};
+
+// 8 values as they lie in memory
+template <typename T>
+struct Raw {
+  uint4 a[sizeof(T) / 2];
 };
 
 // A thread's 8 columns of a row: one run of 8 (VEC) or every G-th column from `tid`.
@@ -47,15 +70,15 @@ struct Cols {
   WB_DEV int at(int k) const { return VEC ? c + k : c + k * G; }
   WB_DEV bool on(int k) const { return at(k) < cols; }
   template <typename T>
-  WB_DEV void load(const T* p, float* v) const {
+  WB_DEV void fetch(const T* p, Raw<T>& r) const {
     if (VEC) {
-      if (on(0)) load8(p + c, v);
-      else
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = 0.f;
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+        r.a[i] = on(0) ? __ldg(reinterpret_cast<const uint4*>(p + c) + i) : make_uint4(0, 0, 0, 0);
     } else {
+      T* v = reinterpret_cast<T*>(r.a);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = on(k) ? to_float(p[at(k)]) : 0.f;
+      for (int k = 0; k < 8; ++k) v[k] = on(k) ? p[at(k)] : from_float<T>(0.f);
     }
   }
   WB_DEV void vector(const float* p, float* v, float none) const {  // a parameter vector, or `none` without one
@@ -73,6 +96,12 @@ struct Cols {
     }
   }
 };
+template <typename T>
+WB_DEV void widen(const Raw<T>& r, float* v) {
+  const T* p = reinterpret_cast<const T*>(r.a);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = to_float(p[k]);
+}
 
 // v <- (v - mean) / sigma in place; returns 1 / sigma.  The variance is taken from the centred values
 // (a second sum), not as a difference of two large sums.
@@ -82,14 +111,14 @@ WB_DEV float normalise(float* v, int kind, const Cols<VEC>& cc, float inv_cols, 
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) s += v[k];
-    const float mean = sum(s, 0.f).x * inv_cols;
+    const float mean = sum(s) * inv_cols;
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = cc.on(k) ? v[k] - mean : 0.f;
   }
   float q = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) q += v[k] * v[k];
-  const float inv = rsqrtf(sum(q, 0.f).x * inv_cols + eps);
+  const float inv = rsqrtf(sum(q) * inv_cols + eps);
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] *= inv;
   return inv;
@@ -105,115 +134,132 @@ WB_DEV void normalise_backward(float* g, const float* n, float inv, int kind, co
     s += g[k];
     p += g[k] * n[k];
   }
-  const float2 t = sum(s, p);
-  const float mg = kind == WUBU_B200_NORM_LAYER ? t.x * inv_cols : 0.f, mp = t.y * inv_cols;
+  const float2 t = kind == WUBU_B200_NORM_LAYER ? sum(s, p) : make_float2(0.f, sum(p));
+  const float mg = t.x * inv_cols, mp = t.y * inv_cols;
 #pragma unroll
   for (int k = 0; k < 8; ++k) g[k] = cc.on(k) ? (g[k] - mg - n[k] * mp) * inv : 0.f;
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(1024) resnorm_forward_kernel(const WubuB200ResNorm a, long long rows) {
-  extern __shared__ float2 red[];
-  const int G = blockDim.x, R = blockDim.y;
-  RowReduce sum{red, G / 32, R, (int)threadIdx.y, (int)threadIdx.x / 32, (int)threadIdx.x & 31, 0};
-  const Cols<VEC> cc{VEC ? (int)threadIdx.x * 8 : (int)threadIdx.x, a.cols, G};
-  const float inv_cols = 1.f / (float)a.cols;
-  const long long row = (long long)blockIdx.x * R + threadIdx.y;
-  const bool on = row < rows;
-  const long long at = on ? row : rows - 1;  // the last block's idle groups repeat the last row, unstored
-  float x[8], f[8], t[8];
-  cc.load(static_cast<const T*>(a.x) + at * a.x_stride, x);
-  cc.load(static_cast<const T*>(a.f) + at * a.f_stride, f);
-  if (a.post) {
-    normalise(f, a.post, cc, inv_cols, a.eps, sum);
-    cc.vector(a.post_weight, t, 1.f);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] *= t[k];
-    cc.vector(a.post_bias, t, 0.f);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] += t[k];
-  }
-  if (a.gate) {
-    cc.vector(a.gate_values + (a.gate == WUBU_B200_GATE_ITEM ? at / a.rows_per_item * a.cols : 0), t, 0.f);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] *= t[k];
-  }
-#pragma unroll
-  for (int k = 0; k < 8; ++k) x[k] = fmaf(a.res_scale, x[k], f[k]);
-  if (a.r && on) cc.store(static_cast<T*>(a.r) + at * a.cols, x);
-  if (!a.norm) return;
-  normalise(x, a.norm, cc, inv_cols, a.eps, sum);
-  cc.vector(a.weight, t, 1.f);
-#pragma unroll
-  for (int k = 0; k < 8; ++k) x[k] *= t[k];
-  cc.vector(a.bias, t, 0.f);
-#pragma unroll
-  for (int k = 0; k < 8; ++k) x[k] += t[k];
-  if (on) cc.store(static_cast<T*>(a.h) + at * a.cols, x);
-}
-
-// The column sums a block hands on, in this order; partials are [vector][block][cols].
-enum { kDWeight, kDBias, kDPostWeight, kDPostBias, kDGate, kVectors };
-
+// A block's rows [t0, t1) of one item.
 struct ResNormGrid {
   int blocks_per_item, rows_per_block;
   long long blocks;
   float* part;
 };
 
-// MAXT: 256 threads may use all the registers that the sums and the row want; rows of more than 2048
-// columns take up to 1024 threads.
+// MAXT: rows of more than kThreads * 8 columns take up to 1024 threads.
 template <typename T, bool VEC, int MAXT>
-__global__ void __launch_bounds__(MAXT) resnorm_backward_kernel(const WubuB200ResNorm a, const ResNormGrid gr) {
+__global__ void __launch_bounds__(MAXT, MAXT == kThreads ? 2 : 1)
+resnorm_forward_kernel(const WubuB200ResNorm a, const ResNormGrid gr) {
   extern __shared__ float2 red[];
   const int G = blockDim.x, R = blockDim.y;
   RowReduce sum{red, G / 32, R, (int)threadIdx.y, (int)threadIdx.x / 32, (int)threadIdx.x & 31, 0};
   const Cols<VEC> cc{VEC ? (int)threadIdx.x * 8 : (int)threadIdx.x, a.cols, G};
   const float inv_cols = 1.f / (float)a.cols;
-  const long long item = blockIdx.x / gr.blocks_per_item;
-  const long long t0 = (long long)(blockIdx.x - item * gr.blocks_per_item) * gr.rows_per_block;
-  const long long t1 = min(t0 + gr.rows_per_block, a.rows_per_item);
-  const float* gate = a.gate ? a.gate_values + (a.gate == WUBU_B200_GATE_ITEM ? item * a.cols : 0) : nullptr;
+  const int item = blockIdx.x / gr.blocks_per_item;
+  const int t0 = (int)(blockIdx.x - item * gr.blocks_per_item) * gr.rows_per_block + threadIdx.y;
+  const int t1 = (int)min((long long)t0 - threadIdx.y + gr.rows_per_block, a.rows_per_item);
+  const long long row0 = item * a.rows_per_item;
+  const T *xp = static_cast<const T*>(a.x), *fp = static_cast<const T*>(a.f);
+  Raw<T> rx, rf;
+  if (t0 < t1) {
+    cc.fetch(xp + (row0 + t0) * a.x_stride, rx);
+    cc.fetch(fp + (row0 + t0) * a.f_stride, rf);
+  }
+  float w[8], wb_[8], pw[8], pb[8];
+  cc.vector(a.weight, w, 1.f);
+  cc.vector(a.bias, wb_, 0.f);
+  cc.vector(a.post_weight, pw, 1.f);
+  cc.vector(a.post_bias, pb, 0.f);
+  if (a.gate) {  // folded into the affine form: gate * (n pw + pb)
+    float gt[8];
+    cc.vector(a.gate_values + (a.gate == WUBU_B200_GATE_ITEM ? (long long)item * a.cols : 0), gt, 0.f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      pw[k] *= gt[k];
+      pb[k] *= gt[k];
+    }
+  }
+  for (int t = t0; t < t1; t += R) {
+    const long long row = row0 + t;
+    float x[8], f[8];
+    widen(rx, x);
+    widen(rf, f);
+    if (t + R < t1) {
+      cc.fetch(xp + (row + R) * a.x_stride, rx);
+      cc.fetch(fp + (row + R) * a.f_stride, rf);
+    }
+    if (a.post) normalise(f, a.post, cc, inv_cols, a.eps, sum);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = fmaf(a.res_scale, x[k], fmaf(f[k], pw[k], pb[k]));
+    if (a.r) cc.store(static_cast<T*>(a.r) + row * a.cols, x);
+    if (!a.norm) continue;
+    normalise(x, a.norm, cc, inv_cols, a.eps, sum);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = fmaf(x[k], w[k], wb_[k]);
+    cc.store(static_cast<T*>(a.h) + row * a.cols, x);
+  }
+}
+
+// The column sums a block hands on, in this order; partials are [vector][block][cols].
+enum { kDWeight, kDBias, kDPostWeight, kDPostBias, kDGate, kVectors };
+
+// POST, GATE: without a post norm or a gate their vectors and sums take no registers (true also serves
+// their absence).
+template <typename T, bool VEC, int MAXT, bool POST, bool GATE>
+__global__ void __launch_bounds__(MAXT, 1) resnorm_backward_kernel(const WubuB200ResNorm a, const ResNormGrid gr) {
+  extern __shared__ float2 red[];
+  const int G = blockDim.x, R = blockDim.y;
+  RowReduce sum{red, G / 32, R, (int)threadIdx.y, (int)threadIdx.x / 32, (int)threadIdx.x & 31, 0};
+  const Cols<VEC> cc{VEC ? (int)threadIdx.x * 8 : (int)threadIdx.x, a.cols, G};
+  const float inv_cols = 1.f / (float)a.cols;
+  const int item = blockIdx.x / gr.blocks_per_item;
+  const int t0 = (int)(blockIdx.x - item * gr.blocks_per_item) * gr.rows_per_block + threadIdx.y;
+  const int t1 = (int)min((long long)t0 - threadIdx.y + gr.rows_per_block, a.rows_per_item);
+  const long long row0 = item * a.rows_per_item;
+  const T *xp = static_cast<const T*>(a.x), *fp = static_cast<const T*>(a.f), *dp = static_cast<const T*>(a.dr),
+          *hp = static_cast<const T*>(a.dh);
+  const bool norm = a.norm && hp;
+  Raw<T> rx, rf, rd, rh;
+  auto fetch = [&](long long row) {
+    cc.fetch(xp + row * a.x_stride, rx);
+    cc.fetch(fp + row * a.f_stride, rf);
+    if (dp) cc.fetch(dp + row * a.dr_stride, rd);
+    if (hp) cc.fetch(hp + row * a.dh_stride, rh);
+  };
+  if (t0 < t1) fetch(row0 + t0);
+  float w[8], pw[8], pb[8], gt[8];
+  cc.vector(a.weight, w, 1.f);
+  if (POST) {
+    cc.vector(a.post_weight, pw, 1.f);
+    cc.vector(a.post_bias, pb, 0.f);
+  }
+  if (GATE) cc.vector(a.gate ? a.gate_values + (a.gate == WUBU_B200_GATE_ITEM ? (long long)item * a.cols : 0) : nullptr, gt, 1.f);
   float dw[8], db[8], dpw[8], dpb[8], dg[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) dw[k] = db[k] = dpw[k] = dpb[k] = dg[k] = 0.f;
-  for (long long t = t0; t < t1; t += R) {  // the same count for all groups of the block (barriers inside)
-    const bool on = t + threadIdx.y < t1;
-    const long long row = item * a.rows_per_item + (on ? t + threadIdx.y : t);
-    float x[8], n[8], d[8], g[8], v[8];
-    cc.load(static_cast<const T*>(a.x) + row * a.x_stride, x);
-    cc.load(static_cast<const T*>(a.f) + row * a.f_stride, n);
+  for (int t = t0; t < t1; t += R) {
+    const long long row = row0 + t;
+    float x[8], n[8], d[8], g[8];
+    widen(rx, x);
+    widen(rf, n);
 #pragma unroll
     for (int k = 0; k < 8; ++k) d[k] = g[k] = 0.f;
-    if (a.dr) cc.load(static_cast<const T*>(a.dr) + row * a.dr_stride, d);
-    if (a.dh) cc.load(static_cast<const T*>(a.dh) + row * a.dh_stride, g);
-    // forward again: n = normalised f, u = its affine form, x <- r <- normalised r
-    const float post_inv = a.post ? normalise(n, a.post, cc, inv_cols, a.eps, sum) : 1.f;
-    float u[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) u[k] = n[k];
-    if (a.post) {
-      cc.vector(a.post_weight, v, 1.f);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) u[k] *= v[k];
-      cc.vector(a.post_bias, v, 0.f);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) u[k] += v[k];
-    }
-    cc.vector(gate, v, 1.f);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = fmaf(a.res_scale, x[k], v[k] * u[k]);
+    if (dp) widen(rd, d);
+    if (hp) widen(rh, g);
+    if (t + R < t1) fetch(row + R);
+    // forward again: n = normalised f, x <- r <- normalised r
+    const float post_inv = POST && a.post ? normalise(n, a.post, cc, inv_cols, a.eps, sum) : 1.f;
+    auto u = [&](int k) { return POST ? fmaf(n[k], pw[k], pb[k]) : n[k]; };
     // d <- gradient of r
-    if (a.norm && a.dh) {
+    if (norm) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = fmaf(a.res_scale, x[k], GATE ? gt[k] * u(k) : u(k));
       const float inv = normalise(x, a.norm, cc, inv_cols, a.eps, sum);
-      float w[8];
-      cc.vector(a.weight, w, 1.f);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        if (on) {
-          dw[k] += g[k] * x[k];
-          db[k] += g[k];
-        }
+        dw[k] += g[k] * x[k];
+        db[k] += g[k];
         g[k] *= w[k];
       }
       normalise_backward(g, x, inv, a.norm, cc, inv_cols, sum);
@@ -224,23 +270,22 @@ __global__ void __launch_bounds__(MAXT) resnorm_backward_kernel(const WubuB200Re
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       x[k] = a.res_scale * d[k];
-      if (on) dg[k] += d[k] * u[k];
-      d[k] *= v[k];
+      if (GATE) {
+        dg[k] += d[k] * u(k);
+        d[k] *= gt[k];
+      }
     }
-    if (a.dx && on) cc.store(static_cast<T*>(a.dx) + row * a.cols, x);
-    if (a.post) {
-      cc.vector(a.post_weight, v, 1.f);
+    if (a.dx) cc.store(static_cast<T*>(a.dx) + row * a.cols, x);
+    if (POST && a.post) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        if (on) {
-          dpw[k] += d[k] * n[k];
-          dpb[k] += d[k];
-        }
-        d[k] *= v[k];
+        dpw[k] += d[k] * n[k];
+        dpb[k] += d[k];
+        d[k] *= pw[k];
       }
       normalise_backward(d, n, post_inv, a.post, cc, inv_cols, sum);
     }
-    if (a.df && on) cc.store(static_cast<T*>(a.df) + row * a.cols, d);
+    if (a.df) cc.store(static_cast<T*>(a.df) + row * a.cols, d);
   }
   // the block's R groups in order, then one partial row per block
   float* acc = reinterpret_cast<float*>(red);
@@ -269,26 +314,27 @@ __global__ void __launch_bounds__(MAXT) resnorm_backward_kernel(const WubuB200Re
   }
 }
 
-// out[item][c] = sum over `n` partial rows from item * n on, in order (8 threads a column, each a run of
-// rows, then the 8 in order).
-constexpr int kReduceCols = 32, kReduceRuns = 8;
+// out[item][c] = sum over `n` partial rows from item * n on, in order (32 threads a column, each a run of
+// rows, then the 32 in order).
+constexpr int kReduceCols = 32, kReduceRuns = 32;
 struct ColumnSums {
   const float* part[kVectors];
   float* out[kVectors];
-  long long n[kVectors];
-  int items[kVectors];
+  int n[kVectors], items[kVectors];
 };
 __global__ void __launch_bounds__(kReduceCols* kReduceRuns) resnorm_sums_kernel(const ColumnSums s, int cols) {
-  __shared__ float run[kReduceRuns][kReduceCols];
+  __shared__ float run[kReduceRuns][kReduceCols + 1];
   const int q = blockIdx.z;
   if ((int)blockIdx.y >= s.items[q]) return;
   const int c = blockIdx.x * kReduceCols + threadIdx.x;
-  const long long n = s.n[q], per = (n + kReduceRuns - 1) / kReduceRuns;
-  const long long i0 = min(n, per * threadIdx.y), i1 = min(n, i0 + per);
+  const int n = s.n[q], per = (n + kReduceRuns - 1) / kReduceRuns;
+  const int i0 = min(n, per * (int)threadIdx.y), i1 = min(n, i0 + per);
   const float* p = s.part[q] + (long long)blockIdx.y * n * cols + c;
   float acc = 0.f;
-  if (c < cols)
-    for (long long i = i0; i < i1; ++i) acc += p[i * cols];
+  if (c < cols) {
+#pragma unroll 8
+    for (int i = i0; i < i1; ++i) acc += __ldg(p + (long long)i * cols);
+  }
   run[threadIdx.y][threadIdx.x] = acc;
   __syncthreads();
   if (threadIdx.y || c >= cols) return;
@@ -320,18 +366,18 @@ int check_resnorm(const WubuB200ResNorm* a) {
 
 bool vec_ok(const WubuB200ResNorm& a, const void* p, long long stride) { return aligned16(p) && stride % 8 == 0; }
 
-// threads a row (a multiple of 32), rows at a time
+// threads a row (a multiple of 32), rows at a time (a barrier each: at most 15)
 dim3 group_of(int cols) {
   const int G = (((cols + 7) / 8) + 31) / 32 * 32;
-  return dim3(G, G >= 128 ? 1 : 128 / G);
+  const int R = G >= kThreads ? 1 : kThreads / G;
+  return dim3(G, R);
 }
 
-// Row ranges of the backward's blocks: enough blocks to fill the SMs several times over, few enough
-// that their partial sums stay small beside the tensors.
-ResNormGrid grid_of(const WubuB200ResNorm& a, const dim3& g) {
-  const long long want = 148 * 4;
+// Row ranges of the blocks: as many blocks as run at once (`resident` an SM), within an item.
+ResNormGrid grid_of(const WubuB200ResNorm& a, const dim3& g, int resident) {
+  const long long want = 148 * resident;
   ResNormGrid r{};
-  long long per_item = (want + a.items - 1) / a.items;
+  long long per_item = want / a.items;
   const long long most = (a.rows_per_item + g.y - 1) / g.y;
   per_item = per_item < 1 ? 1 : per_item > most ? most : per_item;
   long long rows = (a.rows_per_item + per_item - 1) / per_item;
@@ -361,12 +407,14 @@ int wubu_b200_resnorm_forward(const WubuB200ResNorm* p, void* stream) {
   const bool vec = a.cols % 8 == 0 && vec_ok(a, a.x, a.x_stride) && vec_ok(a, a.f, a.f_stride) && aligned16(a.r) &&
                    aligned16(a.h);
   const dim3 g = group_of(a.cols);
-  const unsigned grid = (unsigned)((rows + g.y - 1) / g.y);
+  const ResNormGrid gr = grid_of(a, g, g.x * g.y <= kThreads ? 2 : 1);
+  const size_t smem = reduce_bytes(g);
   cudaStream_t st = (cudaStream_t)stream;
   with_dtype(a.dtype, [&](auto t) {
     typedef decltype(t) T;
-    if (vec) resnorm_forward_kernel<T, true><<<grid, g, reduce_bytes(g), st>>>(a, rows);
-    else resnorm_forward_kernel<T, false><<<grid, g, reduce_bytes(g), st>>>(a, rows);
+    auto* kernel = g.x <= kThreads ? (vec ? resnorm_forward_kernel<T, true, kThreads> : resnorm_forward_kernel<T, false, kThreads>)
+                                   : (vec ? resnorm_forward_kernel<T, true, 1024> : resnorm_forward_kernel<T, false, 1024>);
+    kernel<<<(unsigned)gr.blocks, g, smem, st>>>(a, gr);
   });
   return ops_launched("resnorm_forward");
 }
@@ -374,7 +422,7 @@ int wubu_b200_resnorm_forward(const WubuB200ResNorm* p, void* stream) {
 long long wubu_b200_resnorm_workspace(const WubuB200ResNorm* a) {
   const int rc = check_resnorm(a);
   if (rc != WUBU_B200_OK) return rc == 1 ? 0 : rc;
-  return grid_of(*a, group_of(a->cols)).blocks * kVectors * a->cols * (long long)sizeof(float);
+  return grid_of(*a, group_of(a->cols), 1).blocks * kVectors * a->cols * (long long)sizeof(float);
 }
 
 int wubu_b200_resnorm_backward(const WubuB200ResNorm* p, void* stream) {
@@ -395,7 +443,7 @@ int wubu_b200_resnorm_backward(const WubuB200ResNorm* p, void* stream) {
       !strides_ok(a, a.dh_stride, a.dh))
     return WUBU_B200_ERR_ARG;
   const dim3 g = group_of(a.cols);
-  ResNormGrid gr = grid_of(a, g);
+  ResNormGrid gr = grid_of(a, g, 1);
   bool sums = false;
   for (int q = 0; q < kVectors; ++q) sums = sums || out[q];
   if (sums) {
@@ -411,8 +459,13 @@ int wubu_b200_resnorm_backward(const WubuB200ResNorm* p, void* stream) {
   if (g.y > 1 && smem < sizeof(float) * g.y * a.cols) smem = sizeof(float) * g.y * a.cols;
   with_dtype(a.dtype, [&](auto t) {
     typedef decltype(t) T;
-    auto* kernel = g.x <= 256 ? (vec ? resnorm_backward_kernel<T, true, 256> : resnorm_backward_kernel<T, false, 256>)
-                              : (vec ? resnorm_backward_kernel<T, true, 1024> : resnorm_backward_kernel<T, false, 1024>);
+    auto pick = [&](auto v) {
+      constexpr bool V = decltype(v)::value;
+      if (g.x > kThreads) return resnorm_backward_kernel<T, V, 1024, true, true>;  // (gate and post may be absent)
+      if (a.post) return a.gate ? resnorm_backward_kernel<T, V, kThreads, true, true> : resnorm_backward_kernel<T, V, kThreads, true, false>;
+      return a.gate ? resnorm_backward_kernel<T, V, kThreads, false, true> : resnorm_backward_kernel<T, V, kThreads, false, false>;
+    };
+    auto* kernel = vec ? pick(std::true_type()) : pick(std::false_type());
     kernel<<<(unsigned)gr.blocks, g, smem, st>>>(a, gr);
   });
   rc = ops_launched("resnorm_backward");
@@ -425,7 +478,7 @@ int wubu_b200_resnorm_backward(const WubuB200ResNorm* p, void* stream) {
     s.part[q] = gr.part + (long long)q * gr.blocks * a.cols;
     s.out[q] = out[q];
     s.items[q] = by_item ? (int)a.items : 1;
-    s.n[q] = by_item ? gr.blocks_per_item : gr.blocks;
+    s.n[q] = by_item ? gr.blocks_per_item : (int)gr.blocks;
     if (s.items[q] > items) items = s.items[q];
   }
   resnorm_sums_kernel<<<dim3((a.cols + kReduceCols - 1) / kReduceCols, items, kVectors), dim3(kReduceCols, kReduceRuns),

@@ -15,6 +15,7 @@ first); ``ops_sync`` reports what an asynchronous call could not.
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 from typing import NamedTuple
 
@@ -67,32 +68,37 @@ def _dtype(t, what):
 
 
 def _cuda(what, *ts):
-    dev = ts[0].device
-    if dev.type != "cuda":
+    """The index of the device that all of ``ts`` (None left out) are on."""
+    dev = ts[0].get_device()
+    if dev < 0:
         raise ValueError(f"{what}: CUDA tensors only")
     for t in ts[1:]:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{what}: tensors on cuda:{dev} and {t.device}")
     return dev
 
 
-class _on:
-    """The library launches on the current device: makes ``dev`` current where it is not."""
-
-    def __init__(self, dev):
-        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
+# the current stream's handle without a torch.cuda.Stream object around it, where torch has that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
-def _stream(dev):
-    return torch.cuda.current_stream(dev).cuda_stream
+def _call(what, fn, dev, *args):
+    """fn(*args, current stream of dev) with dev current (the library launches on the current device)."""
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc:
+        _check(rc, what)
+
+
+def _empty(like, dtype=None):
+    """A contiguous tensor of like's shape."""
+    if like.is_contiguous():
+        return torch.empty_like(like, dtype=dtype)
+    return like.new_empty(like.shape, dtype=dtype)
 
 
 def _ptr(t):
@@ -126,9 +132,8 @@ def _rows(t):
 
 def ops_sync(device=None):
     """Waits for the current stream and raises if a kernel of these operators gave up on a wait."""
-    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    with _on(dev):
-        _check(L().wubu_b200_ops_sync(_stream(dev)), "ops_sync")
+    dev = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    _call("ops_sync", L().wubu_b200_ops_sync, dev)
 
 
 # ---- activation with an 8-bit checkpoint of its input --------------------------------------------
@@ -156,12 +161,11 @@ def act8_forward(x, act="gelu", slope=0.0, with_output=True):
     x, step = _rows(x)
     C = x.shape[-1]
     rows = x.numel() // C if C else 0
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev) if with_output else None
-    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
-    scale = torch.empty((*x.shape[:-1], -(-C // ACT8_BLOCK)), dtype=torch.float32, device=dev)
-    with _on(dev):
-        _check(L().wubu_b200_act8_forward(d, _ACTS[act], slope, x.data_ptr(), step, _ptr(y), q.data_ptr(),
-                                          scale.data_ptr(), rows, C, _stream(dev)), "act8_forward")
+    y = _empty(x) if with_output else None
+    q = _empty(x, torch.int8)
+    scale = x.new_empty((*x.shape[:-1], -(-C // ACT8_BLOCK)), dtype=torch.float32)
+    _call("act8_forward", L().wubu_b200_act8_forward, dev, d, _ACTS[act], slope, x.data_ptr(), step, _ptr(y),
+          q.data_ptr(), scale.data_ptr(), rows, C)
     return y, Kept8(q, scale, act, float(slope), x.dtype)
 
 
@@ -177,13 +181,11 @@ def act8_backward(dy, kept, recompute=False):
     step, dx, y = 0, None, None
     if dy is not None:
         dy, step = _rows(dy)
-        dx = torch.empty(q.shape, dtype=kept.dtype, device=dev)
+        dx = torch.empty_like(q, dtype=kept.dtype)
     if recompute or dy is None:
-        y = torch.empty(q.shape, dtype=kept.dtype, device=dev)
-    with _on(dev):
-        _check(L().wubu_b200_act8_backward(_DTYPES[kept.dtype], _ACTS[kept.act], kept.slope, _ptr(dy), step,
-                                           q.data_ptr(), scale.data_ptr(), _ptr(dx), _ptr(y), rows, C, _stream(dev)),
-               "act8_backward")
+        y = torch.empty_like(q, dtype=kept.dtype)
+    _call("act8_backward", L().wubu_b200_act8_backward, dev, _DTYPES[kept.dtype], _ACTS[kept.act], kept.slope, _ptr(dy),
+          step, q.data_ptr(), scale.data_ptr(), _ptr(dx), _ptr(y), rows, C)
     return dx, y
 
 
@@ -200,10 +202,10 @@ _RESNORM = struct.Struct("@4i2qi2fi" + "4q" + "4P" + "P" + "2P" + "4q" + "2P" + 
 def _vector(v, shape, dev, what):
     if v is None:
         return None
-    if tuple(v.shape) != shape:
+    if v.shape != shape:
         raise ValueError(f"{what}: shape {shape}, got {tuple(v.shape)}")
-    if v.device != dev:
-        raise ValueError(f"{what}: tensors on {dev} and {v.device}")
+    if v.get_device() != dev:
+        raise ValueError(f"{what}: tensors on cuda:{dev} and {v.device}")
     if v.dtype != torch.float32 or not v.is_contiguous():
         v = v.to(torch.float32).contiguous()
     return v
@@ -221,12 +223,11 @@ def _resnorm_operands(what, x, f, norm, weight, bias, post, post_weight, post_bi
     dev = _cuda(what, x, f)
     items, C = x.shape[0], x.shape[-1]
     rows = x.numel() // (items * C) if items and C else 0
-    vec = [_vector(v, (C,), dev, what + " " + n) for v, n in
-           ((weight, "weight"), (bias, "bias"), (post_weight, "post_weight"), (post_bias, "post_bias"))]
+    vec = [v if v is None else _vector(v, (C,), dev, what) for v in (weight, bias, post_weight, post_bias)]
     kind = 0
     if gate is not None:
         kind = 1 if gate.dim() == 1 else 2
-        gate = _vector(gate, (C,) if kind == 1 else (items, C), dev, what + " gate")
+        gate = _vector(gate, (C,) if kind == 1 else (items, C), dev, what)
     return dev, items, rows, C, vec, kind, gate
 
 
@@ -242,13 +243,12 @@ def resnorm_forward(x, f, *, norm="layer", weight=None, bias=None, post=None, po
                                                              post_weight, post_bias, gate)
     x, xs = _rows(x)
     f, fs = _rows(f)
-    r = torch.empty(x.shape, dtype=x.dtype, device=dev) if keep_sum else None
-    h = torch.empty(x.shape, dtype=x.dtype, device=dev) if norm else None
+    r = _empty(x) if keep_sum else None
+    h = _empty(x) if norm else None
     args = _RESNORM.pack(d, _NORMS[norm], _NORMS[post], kind, items, rows, C, res_scale, eps, 0, x.data_ptr(), xs,
                          f.data_ptr(), fs, *map(_ptr, vec), _ptr(gate), _ptr(r), _ptr(h), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
                          0, 0, 0)
-    with _on(dev):
-        _check(L().wubu_b200_resnorm_forward(args, _stream(dev)), "resnorm_forward")
+    _call("resnorm_forward", L().wubu_b200_resnorm_forward, dev, args)
     return r, h
 
 
@@ -266,7 +266,7 @@ def resnorm_backward(dr, dh, x, f, *, norm="layer", weight=None, bias=None, post
     for i, t in enumerate(grads):
         if t is None:
             continue
-        if t.shape != x.shape or t.dtype != x.dtype or t.device != dev:
+        if t.shape != x.shape or t.dtype != x.dtype or t.get_device() != dev:
             raise ValueError(f"{what}: dr and dh have x's shape, type and device")
         grads[i], strides[i] = _rows(t)
     if dr is None and dh is None:
@@ -276,10 +276,9 @@ def resnorm_backward(dr, dh, x, f, *, norm="layer", weight=None, bias=None, post
     dr, dh = grads
     x, xs = _rows(x)
     f, fs = _rows(f)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    df = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    like = lambda v: None if v is None else torch.empty(v.shape, dtype=torch.float32, device=dev)  # noqa: E731
-    dweight, dbias, dpost_weight, dpost_bias, dgate = (like(v) for v in (*vec, gate))
+    dx = _empty(x)
+    df = _empty(x)
+    dweight, dbias, dpost_weight, dpost_bias, dgate = (v if v is None else torch.empty_like(v) for v in (*vec, gate))
 
     def pack(ws, n):
         return _RESNORM.pack(d, _NORMS[norm], _NORMS[post], kind, items, rows, C, res_scale, eps, 0, x.data_ptr(), xs,
@@ -288,10 +287,9 @@ def resnorm_backward(dr, dh, x, f, *, norm="layer", weight=None, bias=None, post
                              _ptr(dpost_bias), _ptr(dweight), _ptr(dbias), ws, n)
 
     h = L()
-    with _on(dev):
-        n = _check(h.wubu_b200_resnorm_workspace(pack(0, 0)), what)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        _check(h.wubu_b200_resnorm_backward(pack(ws.data_ptr(), n), _stream(dev)), what)
+    n = _check(h.wubu_b200_resnorm_workspace(pack(0, 0)), what)
+    ws = x.new_empty(n, dtype=torch.uint8)
+    _call(what, h.wubu_b200_resnorm_backward, dev, pack(ws.data_ptr(), n))
     return {"dx": dx, "df": df, "dgate": dgate, "dweight": dweight, "dbias": dbias, "dpost_weight": dpost_weight,
             "dpost_bias": dpost_bias}
 
@@ -319,8 +317,8 @@ def _view(t):
 def _lens(n, B, dev, what):
     if n is None:
         return None
-    if n.shape != (B,) or n.device != dev:
-        raise ValueError(f"{what}: lengths are [{B}] on {dev}, got {tuple(n.shape)} on {n.device}")
+    if n.shape != (B,) or n.get_device() != dev:
+        raise ValueError(f"{what}: lengths are [{B}] on cuda:{dev}, got {tuple(n.shape)} on {n.device}")
     if n.dtype != torch.int32 or not n.is_contiguous():
         n = n.to(torch.int32).contiguous()
     return n
@@ -346,6 +344,13 @@ def _attn_operands(what, q, k, v, causal, window, scale, q_lens, k_lens):
     return dev, head, (_ptr(ql), _ptr(kl)), (ql, kl)
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace(head, backward):
+    """Workspace bytes of a call's sizes (the library's answer depends on nothing else)."""
+    return _check(L().wubu_b200_attn_workspace(_ATTN.pack(*head, 0, 0, *_NO_VIEW * 4, 0, *_NO_VIEW * 4, 0, 0), backward),
+                  "attn_workspace")
+
+
 def attention_forward(q, k, v, *, causal=False, window=0, scale=None, q_lens=None, k_lens=None):
     """``(out, lse)``: softmax(scale q k^T) v over the visible keys, and the float32 log-sum-exp [B, Hq, Tq].
 
@@ -360,14 +365,13 @@ def attention_forward(q, k, v, *, causal=False, window=0, scale=None, q_lens=Non
     k, vk = _view(k)
     v, vv = _view(v)
     B, Tq, Hq, D = q.shape
-    out = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=dev)
-    lse = torch.empty((B, Hq, Tq), dtype=torch.float32, device=dev)
+    out = _empty(q)
+    lse = q.new_empty((B, Hq, Tq), dtype=torch.float32)
     body = (*head, *lens, *vq, *vk, *vv, out.data_ptr(), Tq * Hq * D, Hq * D, D, lse.data_ptr(), *_NO_VIEW * 4)
     h = L()
-    with _on(dev):
-        n = _check(h.wubu_b200_attn_workspace(_ATTN.pack(*body, 0, 0), 0), what)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        _check(h.wubu_b200_attn_forward(_ATTN.pack(*body, _ptr(ws), n), _stream(dev)), what)
+    n = _workspace(head, 0)
+    ws = q.new_empty(n, dtype=torch.uint8) if n else None
+    _call(what, h.wubu_b200_attn_forward, dev, _ATTN.pack(*body, _ptr(ws), n))
     return out, lse
 
 
@@ -378,24 +382,20 @@ def attention_backward(dout, q, k, v, out, lse, *, causal=False, window=0, scale
     dev, head, lens, hold = _attn_operands(what, q, k, v, causal, window, scale, q_lens, k_lens)
     B, Tq, Hq, D = q.shape
     for t in (dout, out):
-        if t.shape != q.shape or t.dtype != q.dtype or t.device != dev:
+        if t.shape != q.shape or t.dtype != q.dtype or t.get_device() != dev:
             raise ValueError(f"{what}: dout and out have q's shape, type and device")
-    if lse.shape != (B, Hq, Tq) or lse.dtype != torch.float32 or lse.device != dev:
+    if lse.shape != (B, Hq, Tq) or lse.dtype != torch.float32 or lse.get_device() != dev:
         raise ValueError(f"{what}: lse is float32 [B, Hq, Tq]")
     lse = lse.contiguous()
     (q, vq), (k, vk), (v, vv), (out, vo), (dout, vg) = map(_view, (q, k, v, out, dout))
     Tk, Hkv = k.shape[1:3]
-    dq = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=dev)
-    dk = torch.empty((B, Tk, Hkv, D), dtype=q.dtype, device=dev)
-    dv = torch.empty((B, Tk, Hkv, D), dtype=q.dtype, device=dev)
+    dq, dk, dv = _empty(q), _empty(k), _empty(v)
     sq, skv = (Tq * Hq * D, Hq * D, D), (Tk * Hkv * D, Hkv * D, D)
     body = (*head, *lens, *vq, *vk, *vv, *vo, lse.data_ptr(), *vg, dq.data_ptr(), *sq, dk.data_ptr(), *skv,
             dv.data_ptr(), *skv)
-    h = L()
-    with _on(dev):
-        n = _check(h.wubu_b200_attn_workspace(_ATTN.pack(*body, 0, 0), 1), what)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        _check(h.wubu_b200_attn_backward(_ATTN.pack(*body, ws.data_ptr(), n), _stream(dev)), what)
+    n = _workspace(head, 1)
+    ws = q.new_empty(n, dtype=torch.uint8)
+    _call(what, L().wubu_b200_attn_backward, dev, _ATTN.pack(*body, ws.data_ptr(), n))
     return dq, dk, dv
 
 
