@@ -8,6 +8,8 @@
 // Both kernels move each byte once and are bound by HBM: forward 2 + 2 + 1 bytes a 16-bit value,
 // backward 1 + 2 + 2 (+ 2 for y').  Eight threads own a block, 16 values each, as two 16-byte pieces
 // 64 values apart, so that a warp's load covers whole 128-byte lines.
+#include <type_traits>
+
 #include "ops.cuh"
 
 namespace wb {
@@ -18,7 +20,6 @@ constexpr int kThreads = 256;
 constexpr float kTiny = 0x1p-100f;  // below this a block is kept as zeros (127 / max|x| must not overflow)
 
 struct Act8 {
-  int act;
   float slope;
   const void* in;  // x (forward) or dy (backward)
   long long in_stride;
@@ -30,53 +31,59 @@ struct Act8 {
   int cols, nblk;
 };
 
-WB_DEV float exp2f_fast(float x) {
+// Approximations of the hardware's function units (relative error near 2^-22).
+WB_DEV float fast_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-
-// Phi(x) and the density phi(x) of the normal distribution from one exponential and one reciprocal:
-// Phi(-|x|) is e^(-x^2/2) times a polynomial in t = 1 / (1 + p |x| / sqrt 2) (Abramowitz and Stegun,
-// Handbook of Mathematical Functions, 7.1.26; absolute error below 1e-7).  Straight-line code: a
-// library erff in two ranges, with expf beside it, made the backward twice as slow as its memory traffic.
-WB_DEV void normal(float x, float& cdf, float& density) {
-  const float z = fabsf(x);
-  const float t = __fdividef(1.f, fmaf(0.3275911f * 0.70710678118654752f, z, 1.f));
-  const float e = exp2f_fast(x * x * -0.72134752044448170f);  // e^(-x^2/2)
-  float s = fmaf(1.061405429f, t, -1.453152027f);
-  s = fmaf(s, t, 1.421413741f);
-  s = fmaf(s, t, -0.284496736f);
-  s = fmaf(s, t, 0.254829592f);
-  const float tail = 0.5f * s * t * e;
-  cdf = x > 0.f ? 1.f - tail : tail;
-  density = e * 0.39894228040143268f;
+WB_DEV float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-WB_DEV float act_value(float x, int act, float slope) {
-  if (act == WUBU_B200_ACT_LRELU) return x > 0.f ? x : slope * x;
-  if (act == WUBU_B200_ACT_GELU) {
-    float cdf, density;
-    normal(x, cdf, density);
-    return x * cdf;
+// Phi(-|x|) and e^(-x^2/2): the first is the second times a polynomial in t = 1 / (1 + p |x| / sqrt 2) (Abramowitz
+// and Stegun, Handbook of Mathematical Functions, 7.1.26, halved; absolute error below 1e-7).
+// Straight-line code with one exponential and one reciprocal: a library erff in two ranges with expf
+// beside it took twice the time of the memory traffic.
+WB_DEV float normal_tail(float x, float& e) {
+  const float t = fast_rcp(fmaf(0.3275911f * 0.70710678118654752f, fabsf(x), 1.f));
+  e = fast_ex2(x * x * -0.72134752044448170f);
+  float s = fmaf(0.5f * 1.061405429f, t, -0.5f * 1.453152027f);
+  s = fmaf(s, t, 0.5f * 1.421413741f);
+  s = fmaf(s, t, -0.5f * 0.284496736f);
+  s = fmaf(s, t, 0.5f * 0.254829592f);
+  return s * t * e;
+}
+
+template <int ACT>
+WB_DEV float act_value(float x, float slope) {
+  if (ACT == WUBU_B200_ACT_LRELU) return x > 0.f ? x : slope * x;
+  if (ACT == WUBU_B200_ACT_GELU) {
+    float e;
+    const float tail = normal_tail(x, e);
+    return fmaf(-fabsf(x), tail, x > 0.f ? x : x * 0.f);  // x Phi(x) = max(x, 0) - |x| Phi(-|x|); NaN stays NaN
   }
-  if (act == WUBU_B200_ACT_SILU) return __fdividef(x, 1.f + __expf(-x));
+  if (ACT == WUBU_B200_ACT_SILU) return x * fast_rcp(1.f + fast_ex2(x * -1.4426950408889634f));
   return x;
 }
 // act(x) and act'(x)
-WB_DEV void act_both(float x, int act, float slope, float& y, float& d) {
-  if (act == WUBU_B200_ACT_LRELU) {
+template <int ACT>
+WB_DEV void act_both(float x, float slope, float& y, float& d) {
+  if (ACT == WUBU_B200_ACT_LRELU) {
     d = x > 0.f ? 1.f : slope;
     y = x * d;
-  } else if (act == WUBU_B200_ACT_GELU) {
-    float cdf, density;
-    normal(x, cdf, density);
+  } else if (ACT == WUBU_B200_ACT_GELU) {
+    float e;
+    const float tail = normal_tail(x, e);
+    const float cdf = 0.5f + copysignf(0.5f - tail, x);
     y = x * cdf;
-    d = fmaf(x, density, cdf);
-  } else if (act == WUBU_B200_ACT_SILU) {
-    const float t = __fdividef(1.f, 1.f + __expf(-x));
+    d = fmaf(x * 0.39894228040143268f, e, cdf);
+  } else if (ACT == WUBU_B200_ACT_SILU) {
+    const float t = fast_rcp(1.f + fast_ex2(x * -1.4426950408889634f));
     y = x * t;
-    d = t * (1.f + x * (1.f - t));
+    d = fmaf(y, 1.f - t, t);
   } else {
     y = x;
     d = 1.f;
@@ -86,6 +93,26 @@ WB_DEV void act_both(float x, int act, float slope, float& y, float& d) {
 // max|x| as float bits: the order of non-negative floats is that of their bits, and infinities and
 // NaN come out above every finite value (a floating-point maximum would drop a NaN).
 WB_DEV uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+// The same of 8 values in memory form; 16-bit values two at a time.
+WB_DEV uint32_t abs_bits8(const uint4* r, float) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    m = max(max(m, r[i].x & 0x7FFFFFFFu), r[i].y & 0x7FFFFFFFu);
+    m = max(max(m, r[i].z & 0x7FFFFFFFu), r[i].w & 0x7FFFFFFFu);
+  }
+  return m;
+}
+WB_DEV uint32_t abs_halves(const uint4* r) {
+  constexpr uint32_t k = 0x7FFF7FFFu;
+  const uint32_t m = __vmaxu2(__vmaxu2(r->x & k, r->y & k), __vmaxu2(r->z & k, r->w & k));
+  return max(m >> 16, m & 0xFFFFu);
+}
+WB_DEV uint32_t abs_bits8(const uint4* r, bf16) { return abs_halves(r) << 16; }
+WB_DEV uint32_t abs_bits8(const uint4* r, f16) {
+  return __float_as_uint(__half2float(__ushort_as_half((unsigned short)abs_halves(r))));
+}
 
 WB_DEV void block_scale(uint32_t top, float& inv, float& scale) {
   const float m = __uint_as_float(top);
@@ -97,37 +124,32 @@ WB_DEV void block_scale(uint32_t top, float& inv, float& scale) {
   }
 }
 
-// round-to-even(x * inv) as an int8: adding 1.5 * 2^23 leaves the integer in the low bits of the float
-WB_DEV uint32_t quantise(float x, float inv) {
-  return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.f)) & 0xFFu;
+// round-to-even(x * inv) as an int8 in the low byte: adding 1.5 * 2^23 leaves the integer in the low bits of
+// the float
+WB_DEV uint32_t quantise(float x, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.f)); }
+WB_DEV uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 // byte k of w, offset by 128, as a float: the byte becomes the low mantissa bits of 2^23
 WB_DEV float dequantise(uint32_t w_offset, int k) {
   return __uint_as_float(__byte_perm(w_offset, 0x4B000000u, 0x7440u | (uint32_t)k)) - 8388736.f;
 }
 
-template <typename T>
+template <typename T, int ACT>
 __global__ void __launch_bounds__(kThreads) act8_forward_kernel(const Act8 a) {
   const int t = threadIdx.x & 7;
   const long long blk = ((long long)blockIdx.x * kThreads + threadIdx.x) >> 3;
   const bool on = blk < a.blocks;
-  const long long row = on ? blk / a.nblk : 0;
+  const long long row = !on ? 0 : a.nblk == 1 ? blk : blk / a.nblk;
   const int c0 = on ? (int)(blk - row * a.nblk) * kBlock + t * 8 : a.cols;
   const T* x = static_cast<const T*>(a.in) + row * a.in_stride;
-  float v[16];
-  uint32_t top = 0;
+  uint4 raw[2][sizeof(T) / 2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float* w = v + 8 * i;
-    if (c0 + 64 * i < a.cols) {
-      load8(x + c0 + 64 * i, w);
-    } else {
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) w[k] = 0.f;
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < 16; ++k) top = max(top, abs_bits(v[k]));
+    for (int k = 0; k < (int)sizeof(T) / 2; ++k)
+      raw[i][k] = c0 + 64 * i < a.cols ? __ldg(reinterpret_cast<const uint4*>(x + c0 + 64 * i) + k) : make_uint4(0, 0, 0, 0);
+  uint32_t top = max(abs_bits8(raw[0], T()), abs_bits8(raw[1], T()));
 #pragma unroll
   for (int m = 1; m < 8; m <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, m));
   if (!on) return;
@@ -138,57 +160,59 @@ __global__ void __launch_bounds__(kThreads) act8_forward_kernel(const Act8 a) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     if (c0 + 64 * i >= a.cols) continue;
-    const float* w = v + 8 * i;
+    float w[8];
+    const T* e = reinterpret_cast<const T*>(raw[i]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = to_float(e[k]);
     const long long at = row * a.cols + c0 + 64 * i;
-    uint32_t lo = 0, hi = 0;
-    if (!bad) {
+    uint32_t q[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        lo |= quantise(w[k], inv) << (8 * k);
-        hi |= quantise(w[k + 4], inv) << (8 * k);
-      }
-    }
-    *reinterpret_cast<uint2*>(a.q + at) = make_uint2(lo, hi);
+    for (int k = 0; k < 8; ++k) q[k] = quantise(w[k], inv);
+    const uint2 packed = make_uint2(low_bytes(q[0], q[1], q[2], q[3]), low_bytes(q[4], q[5], q[6], q[7]));
+    *reinterpret_cast<uint2*>(a.q + at) = bad ? make_uint2(0, 0) : packed;
     if (a.out) {
-      float y[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) y[k] = act_value(w[k], a.act, a.slope);
-      store8(static_cast<T*>(a.out) + at, y);
+      for (int k = 0; k < 8; ++k) w[k] = act_value<ACT>(w[k], a.slope);
+      store8(static_cast<T*>(a.out) + at, w);
     }
   }
 }
 
-template <typename T>
+template <typename T, int ACT>
 __global__ void __launch_bounds__(kThreads) act8_backward_kernel(const Act8 a) {
   const int t = threadIdx.x & 7;
   const long long blk = ((long long)blockIdx.x * kThreads + threadIdx.x) >> 3;
   if (blk >= a.blocks) return;
-  const long long row = blk / a.nblk;
+  const long long row = a.nblk == 1 ? blk : blk / a.nblk;
   const int c0 = (int)(blk - row * a.nblk) * kBlock + t * 8;
   const float scale = __ldg(a.scale + blk);
+  const long long at = row * a.cols + c0;
+  uint2 q[2];
+  float g[2][8];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int c = c0 + 64 * i;
-    if (c >= a.cols) continue;
-    const long long at = row * a.cols + c;
-    const uint2 q = __ldg(reinterpret_cast<const uint2*>(a.q + at));
-    float g[8], y[8];
-    if (a.in) load8(static_cast<const T*>(a.in) + row * a.in_stride + c, g);
-    const uint32_t lo = q.x ^ 0x80808080u, hi = q.y ^ 0x80808080u;
+    if (c0 + 64 * i >= a.cols) continue;
+    q[i] = __ldg(reinterpret_cast<const uint2*>(a.q + at + 64 * i));
+    if (a.in) load8(static_cast<const T*>(a.in) + row * a.in_stride + c0 + 64 * i, g[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (c0 + 64 * i >= a.cols) continue;
+    float y[8];
+    const uint32_t lo = q[i].x ^ 0x80808080u, hi = q[i].y ^ 0x80808080u;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float x = dequantise(k < 4 ? lo : hi, k & 3) * scale;
       float d;
-      act_both(x, a.act, a.slope, y[k], d);
-      g[k] = a.in ? g[k] * d : 0.f;
+      act_both<ACT>(dequantise(k < 4 ? lo : hi, k & 3) * scale, a.slope, y[k], d);
+      g[i][k] *= d;
     }
-    if (a.out) store8(static_cast<T*>(a.out) + at, g);
-    if (a.again) store8(static_cast<T*>(a.again) + at, y);
+    if (a.out) store8(static_cast<T*>(a.out) + at + 64 * i, g[i]);
+    if (a.again) store8(static_cast<T*>(a.again) + at + 64 * i, y);
   }
 }
 
 // Rows whose length, stride or address rules out 16-byte pieces: a warp owns a block, 4 values a lane.
-template <typename T>
+template <typename T, int ACT>
 __global__ void __launch_bounds__(kThreads) act8_forward_any_kernel(const Act8 a) {
   const int lane = threadIdx.x & 31;
   const long long blk = ((long long)blockIdx.x * kThreads + threadIdx.x) >> 5;
@@ -213,11 +237,11 @@ __global__ void __launch_bounds__(kThreads) act8_forward_any_kernel(const Act8 a
     if (c0 + 32 * i >= a.cols) continue;
     const long long at = row * a.cols + c0 + 32 * i;
     a.q[at] = bad ? (signed char)0 : (signed char)quantise(v[i], inv);
-    if (a.out) static_cast<T*>(a.out)[at] = from_float<T>(act_value(v[i], a.act, a.slope));
+    if (a.out) static_cast<T*>(a.out)[at] = from_float<T>(act_value<ACT>(v[i], a.slope));
   }
 }
 
-template <typename T>
+template <typename T, int ACT>
 __global__ void __launch_bounds__(kThreads) act8_backward_any_kernel(const Act8 a) {
   const int lane = threadIdx.x & 31;
   const long long blk = ((long long)blockIdx.x * kThreads + threadIdx.x) >> 5;
@@ -231,12 +255,20 @@ __global__ void __launch_bounds__(kThreads) act8_backward_any_kernel(const Act8 
     if (c >= a.cols) continue;
     const long long at = row * a.cols + c;
     float y, d;
-    act_both((float)a.q[at] * scale, a.act, a.slope, y, d);
+    act_both<ACT>((float)a.q[at] * scale, a.slope, y, d);
     if (a.out)
       static_cast<T*>(a.out)[at] =
           from_float<T>(to_float(static_cast<const T*>(a.in)[row * a.in_stride + c]) * d);
     if (a.again) static_cast<T*>(a.again)[at] = from_float<T>(y);
   }
+}
+
+template <typename F>
+void with_act(int act, F f) {
+  if (act == WUBU_B200_ACT_LRELU) f(std::integral_constant<int, WUBU_B200_ACT_LRELU>());
+  else if (act == WUBU_B200_ACT_GELU) f(std::integral_constant<int, WUBU_B200_ACT_GELU>());
+  else if (act == WUBU_B200_ACT_SILU) f(std::integral_constant<int, WUBU_B200_ACT_SILU>());
+  else f(std::integral_constant<int, WUBU_B200_ACT_IDENTITY>());
 }
 
 // Everything but the pointers; 1 = nothing to do.
@@ -268,15 +300,18 @@ int wubu_b200_act8_forward(int dtype, int act, float slope, const void* x, long 
   const int rc = check_act8(dtype, act, rows, cols);
   if (rc != WUBU_B200_OK) return rc == 1 ? WUBU_B200_OK : rc;
   if (!x || !q || !scale || (rows > 1 && x_stride < cols)) return WUBU_B200_ERR_ARG;
-  Act8 a{act, slope, x, rows > 1 ? x_stride : 0, y, nullptr, q, scale, rows, 0, cols, (cols + kBlock - 1) / kBlock};
+  Act8 a{slope, x, rows > 1 ? x_stride : 0, y, nullptr, q, scale, rows, 0, cols, (cols + kBlock - 1) / kBlock};
   a.blocks = rows * a.nblk;
   cudaStream_t st = (cudaStream_t)stream;
   const int per = whole_pieces(a) ? kThreads / 8 : kThreads / 32;
   const unsigned grid = (unsigned)((a.blocks + per - 1) / per);
   with_dtype(dtype, [&](auto t) {
-    typedef decltype(t) T;
-    if (per == kThreads / 8) act8_forward_kernel<T><<<grid, kThreads, 0, st>>>(a);
-    else act8_forward_any_kernel<T><<<grid, kThreads, 0, st>>>(a);
+    with_act(act, [&](auto k) {
+      typedef decltype(t) T;
+      constexpr int A = decltype(k)::value;
+      if (per == kThreads / 8) act8_forward_kernel<T, A><<<grid, kThreads, 0, st>>>(a);
+      else act8_forward_any_kernel<T, A><<<grid, kThreads, 0, st>>>(a);
+    });
   });
   return ops_launched("act8_forward");
 }
@@ -286,16 +321,19 @@ int wubu_b200_act8_backward(int dtype, int act, float slope, const void* dy, lon
   const int rc = check_act8(dtype, act, rows, cols);
   if (rc != WUBU_B200_OK) return rc == 1 ? WUBU_B200_OK : rc;
   if (!q || !scale || !dy != !dx || (!dx && !y_again) || (dy && rows > 1 && dy_stride < cols)) return WUBU_B200_ERR_ARG;
-  Act8 a{act, slope, dy, dy && rows > 1 ? dy_stride : 0, dx, y_again, const_cast<signed char*>(q),
+  Act8 a{slope, dy, dy && rows > 1 ? dy_stride : 0, dx, y_again, const_cast<signed char*>(q),
          const_cast<float*>(scale), rows, 0, cols, (cols + kBlock - 1) / kBlock};
   a.blocks = rows * a.nblk;
   cudaStream_t st = (cudaStream_t)stream;
   const int per = whole_pieces(a) ? kThreads / 8 : kThreads / 32;
   const unsigned grid = (unsigned)((a.blocks + per - 1) / per);
   with_dtype(dtype, [&](auto t) {
-    typedef decltype(t) T;
-    if (per == kThreads / 8) act8_backward_kernel<T><<<grid, kThreads, 0, st>>>(a);
-    else act8_backward_any_kernel<T><<<grid, kThreads, 0, st>>>(a);
+    with_act(act, [&](auto k) {
+      typedef decltype(t) T;
+      constexpr int A = decltype(k)::value;
+      if (per == kThreads / 8) act8_backward_kernel<T, A><<<grid, kThreads, 0, st>>>(a);
+      else act8_backward_any_kernel<T, A><<<grid, kThreads, 0, st>>>(a);
+    });
   });
   return ops_launched("act8_backward");
 }

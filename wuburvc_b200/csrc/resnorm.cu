@@ -36,8 +36,13 @@ struct RowReduce {  // sums over a row's group of warps; four buffers in turn ne
     turn = (turn + 1) & 3;
     if (lane == 0) mine[warp] = make_float2(a, b);
     asm volatile("bar.sync %0, %1;" ::"r"(row + 1), "r"(warps * 32) : "memory");
-    a = b = 0.f;
-    for (int i = 0; i < warps; ++i) {
+    a = mine[0].x + mine[1].x;
+    b = mine[0].y + mine[1].y;
+    if (warps > 2) {
+      a += mine[2].x;
+      b += mine[2].y;
+    }
+    for (int i = 3; i < warps; ++i) {
       a += mine[i].x;
       b += mine[i].y;
     }
@@ -51,8 +56,9 @@ struct RowReduce {  // sums over a row's group of warps; four buffers in turn ne
     turn = (turn + 1) & 3;
     if (lane == 0) mine[warp].x = a;
     asm volatile("bar.sync %0, %1;" ::"r"(row + 1), "r"(warps * 32) : "memory");
-    a = 0.f;
-    for (int i = 0; i < warps; ++i) a += mine[i].x;
+    a = mine[0].x + mine[1].x;
+    if (warps > 2) a += mine[2].x;
+    for (int i = 3; i < warps; ++i) a += mine[i].x;
     return a;
   }
 };
@@ -67,8 +73,10 @@ struct Raw {
 template <bool VEC>
 struct Cols {
   int c, cols, G;
+  bool any;  // c < cols; with VEC that goes for all 8 (cols is a multiple of 8)
+  WB_DEV Cols(int tid, int cols_, int G_) : c(VEC ? tid * 8 : tid), cols(cols_), G(G_), any(c < cols_) {}
   WB_DEV int at(int k) const { return VEC ? c + k : c + k * G; }
-  WB_DEV bool on(int k) const { return at(k) < cols; }
+  WB_DEV bool on(int k) const { return VEC ? any : at(k) < cols; }
   template <typename T>
   WB_DEV void fetch(const T* p, Raw<T>& r) const {
     if (VEC) {
@@ -154,17 +162,21 @@ resnorm_forward_kernel(const WubuB200ResNorm a, const ResNormGrid gr) {
   extern __shared__ float2 red[];
   const int G = blockDim.x, R = blockDim.y;
   RowReduce sum{red, G / 32, R, (int)threadIdx.y, (int)threadIdx.x / 32, (int)threadIdx.x & 31, 0};
-  const Cols<VEC> cc{VEC ? (int)threadIdx.x * 8 : (int)threadIdx.x, a.cols, G};
+  const Cols<VEC> cc((int)threadIdx.x, a.cols, G);
   const float inv_cols = 1.f / (float)a.cols;
   const int item = blockIdx.x / gr.blocks_per_item;
   const int t0 = (int)(blockIdx.x - item * gr.blocks_per_item) * gr.rows_per_block + threadIdx.y;
   const int t1 = (int)min((long long)t0 - threadIdx.y + gr.rows_per_block, a.rows_per_item);
   const long long row0 = item * a.rows_per_item;
-  const T *xp = static_cast<const T*>(a.x), *fp = static_cast<const T*>(a.f);
+  // the next row to load, and the next to store
+  const T *xp = static_cast<const T*>(a.x) + (row0 + t0) * a.x_stride,
+          *fp = static_cast<const T*>(a.f) + (row0 + t0) * a.f_stride;
+  const long long xs = R * a.x_stride, fs = R * a.f_stride, os = (long long)R * a.cols;
+  T *rp = static_cast<T*>(a.r) + (row0 + t0) * a.cols, *hp = static_cast<T*>(a.h) + (row0 + t0) * a.cols;
   Raw<T> rx, rf;
   if (t0 < t1) {
-    cc.fetch(xp + (row0 + t0) * a.x_stride, rx);
-    cc.fetch(fp + (row0 + t0) * a.f_stride, rf);
+    cc.fetch(xp, rx);
+    cc.fetch(fp, rf);
   }
   float w[8], wb_[8], pw[8], pb[8];
   cc.vector(a.weight, w, 1.f);
@@ -180,24 +192,23 @@ resnorm_forward_kernel(const WubuB200ResNorm a, const ResNormGrid gr) {
       pb[k] *= gt[k];
     }
   }
-  for (int t = t0; t < t1; t += R) {
-    const long long row = row0 + t;
+  for (int t = t0; t < t1; t += R, rp += os, hp += os) {
     float x[8], f[8];
     widen(rx, x);
     widen(rf, f);
     if (t + R < t1) {
-      cc.fetch(xp + (row + R) * a.x_stride, rx);
-      cc.fetch(fp + (row + R) * a.f_stride, rf);
+      cc.fetch(xp += xs, rx);
+      cc.fetch(fp += fs, rf);
     }
     if (a.post) normalise(f, a.post, cc, inv_cols, a.eps, sum);
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = fmaf(a.res_scale, x[k], fmaf(f[k], pw[k], pb[k]));
-    if (a.r) cc.store(static_cast<T*>(a.r) + row * a.cols, x);
+    if (a.r) cc.store(rp, x);
     if (!a.norm) continue;
     normalise(x, a.norm, cc, inv_cols, a.eps, sum);
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = fmaf(x[k], w[k], wb_[k]);
-    cc.store(static_cast<T*>(a.h) + row * a.cols, x);
+    cc.store(hp, x);
   }
 }
 
@@ -211,23 +222,30 @@ __global__ void __launch_bounds__(MAXT, 1) resnorm_backward_kernel(const WubuB20
   extern __shared__ float2 red[];
   const int G = blockDim.x, R = blockDim.y;
   RowReduce sum{red, G / 32, R, (int)threadIdx.y, (int)threadIdx.x / 32, (int)threadIdx.x & 31, 0};
-  const Cols<VEC> cc{VEC ? (int)threadIdx.x * 8 : (int)threadIdx.x, a.cols, G};
+  const Cols<VEC> cc((int)threadIdx.x, a.cols, G);
   const float inv_cols = 1.f / (float)a.cols;
   const int item = blockIdx.x / gr.blocks_per_item;
   const int t0 = (int)(blockIdx.x - item * gr.blocks_per_item) * gr.rows_per_block + threadIdx.y;
   const int t1 = (int)min((long long)t0 - threadIdx.y + gr.rows_per_block, a.rows_per_item);
   const long long row0 = item * a.rows_per_item;
-  const T *xp = static_cast<const T*>(a.x), *fp = static_cast<const T*>(a.f), *dp = static_cast<const T*>(a.dr),
-          *hp = static_cast<const T*>(a.dh);
-  const bool norm = a.norm && hp;
+  const T *xp = static_cast<const T*>(a.x) + (row0 + t0) * a.x_stride,
+          *fp = static_cast<const T*>(a.f) + (row0 + t0) * a.f_stride,
+          *dp = static_cast<const T*>(a.dr) + (row0 + t0) * a.dr_stride,
+          *hp = static_cast<const T*>(a.dh) + (row0 + t0) * a.dh_stride;
+  T *dxp = static_cast<T*>(a.dx) + (row0 + t0) * a.cols, *dfp = static_cast<T*>(a.df) + (row0 + t0) * a.cols;
+  const bool norm = a.norm && a.dh;
   Raw<T> rx, rf, rd, rh;
-  auto fetch = [&](long long row) {
-    cc.fetch(xp + row * a.x_stride, rx);
-    cc.fetch(fp + row * a.f_stride, rf);
-    if (dp) cc.fetch(dp + row * a.dr_stride, rd);
-    if (hp) cc.fetch(hp + row * a.dh_stride, rh);
+  auto fetch = [&] {  // the row at the pointers, which move on
+    cc.fetch(xp, rx);
+    cc.fetch(fp, rf);
+    if (a.dr) cc.fetch(dp, rd);
+    if (a.dh) cc.fetch(hp, rh);
+    xp += R * a.x_stride;
+    fp += R * a.f_stride;
+    dp += R * a.dr_stride;
+    hp += R * a.dh_stride;
   };
-  if (t0 < t1) fetch(row0 + t0);
+  if (t0 < t1) fetch();
   float w[8], pw[8], pb[8], gt[8];
   cc.vector(a.weight, w, 1.f);
   if (POST) {
@@ -238,16 +256,15 @@ __global__ void __launch_bounds__(MAXT, 1) resnorm_backward_kernel(const WubuB20
   float dw[8], db[8], dpw[8], dpb[8], dg[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) dw[k] = db[k] = dpw[k] = dpb[k] = dg[k] = 0.f;
-  for (int t = t0; t < t1; t += R) {
-    const long long row = row0 + t;
+  for (int t = t0; t < t1; t += R, dxp += (long long)R * a.cols, dfp += (long long)R * a.cols) {
     float x[8], n[8], d[8], g[8];
     widen(rx, x);
     widen(rf, n);
 #pragma unroll
     for (int k = 0; k < 8; ++k) d[k] = g[k] = 0.f;
-    if (dp) widen(rd, d);
-    if (hp) widen(rh, g);
-    if (t + R < t1) fetch(row + R);
+    if (a.dr) widen(rd, d);
+    if (a.dh) widen(rh, g);
+    if (t + R < t1) fetch();
     // forward again: n = normalised f, x <- r <- normalised r
     const float post_inv = POST && a.post ? normalise(n, a.post, cc, inv_cols, a.eps, sum) : 1.f;
     auto u = [&](int k) { return POST ? fmaf(n[k], pw[k], pb[k]) : n[k]; };
@@ -275,7 +292,7 @@ __global__ void __launch_bounds__(MAXT, 1) resnorm_backward_kernel(const WubuB20
         d[k] *= gt[k];
       }
     }
-    if (a.dx) cc.store(static_cast<T*>(a.dx) + row * a.cols, x);
+    if (a.dx) cc.store(dxp, x);
     if (POST && a.post) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -285,7 +302,7 @@ __global__ void __launch_bounds__(MAXT, 1) resnorm_backward_kernel(const WubuB20
       }
       normalise_backward(d, n, post_inv, a.post, cc, inv_cols, sum);
     }
-    if (a.df) cc.store(static_cast<T*>(a.df) + row * a.cols, d);
+    if (a.df) cc.store(dfp, d);
   }
   // the block's R groups in order, then one partial row per block
   float* acc = reinterpret_cast<float*>(red);
@@ -314,22 +331,22 @@ __global__ void __launch_bounds__(MAXT, 1) resnorm_backward_kernel(const WubuB20
   }
 }
 
-// out[item][c] = sum over `n` partial rows from item * n on, in order (32 threads a column, each a run of
-// rows, then the 32 in order).
-constexpr int kReduceCols = 32, kReduceRuns = 32;
+// out[c] = sum over n partial rows, in order: 8 threads a column, each a run of rows, then the 8 in order.
+// blockIdx.y counts the sums that are asked for, the gate's one to an item.
+constexpr int kReduceCols = 32, kReduceRuns = 8;
 struct ColumnSums {
   const float* part[kVectors];
   float* out[kVectors];
-  int n[kVectors], items[kVectors];
+  int n[kVectors];
+  int count;  // sums before the last entry, which holds the items' gates
 };
 __global__ void __launch_bounds__(kReduceCols* kReduceRuns) resnorm_sums_kernel(const ColumnSums s, int cols) {
-  __shared__ float run[kReduceRuns][kReduceCols + 1];
-  const int q = blockIdx.z;
-  if ((int)blockIdx.y >= s.items[q]) return;
+  __shared__ float run[kReduceRuns][kReduceCols];
+  const int q = min((int)blockIdx.y, s.count), item = blockIdx.y - q;
   const int c = blockIdx.x * kReduceCols + threadIdx.x;
   const int n = s.n[q], per = (n + kReduceRuns - 1) / kReduceRuns;
   const int i0 = min(n, per * (int)threadIdx.y), i1 = min(n, i0 + per);
-  const float* p = s.part[q] + (long long)blockIdx.y * n * cols + c;
+  const float* p = s.part[q] + (long long)item * n * cols + c;
   float acc = 0.f;
   if (c < cols) {
 #pragma unroll 8
@@ -341,7 +358,7 @@ __global__ void __launch_bounds__(kReduceCols* kReduceRuns) resnorm_sums_kernel(
   acc = 0.f;
 #pragma unroll
   for (int i = 0; i < kReduceRuns; ++i) acc += run[i][threadIdx.x];
-  s.out[q][(long long)blockIdx.y * cols + c] = acc;
+  s.out[q][(long long)item * cols + c] = acc;
 }
 
 bool strides_ok(const WubuB200ResNorm& a, long long stride, const void* p) {
@@ -356,7 +373,7 @@ int check_resnorm(const WubuB200ResNorm* a) {
     return WUBU_B200_ERR_ARG;
   if (a->cols < 1 || a->cols > kMaxCols) return WUBU_B200_ERR_SHAPE;
   if (a->items == 0 || a->rows_per_item == 0) return 1;
-  if (a->rows_per_item > 0x7FFFFFFFll / a->items || (a->gate == WUBU_B200_GATE_ITEM && a->items > 65535))
+  if (a->rows_per_item > 0x7FFFFFFFll / a->items || (a->gate == WUBU_B200_GATE_ITEM && a->items > 65000))
     return WUBU_B200_ERR_SHAPE;
   if (!a->x || !a->f || (a->gate && !a->gate_values) || !strides_ok(*a, a->x_stride, a->x) ||
       !strides_ok(*a, a->f_stride, a->f))
@@ -471,18 +488,18 @@ int wubu_b200_resnorm_backward(const WubuB200ResNorm* p, void* stream) {
   rc = ops_launched("resnorm_backward");
   if (rc != WUBU_B200_OK || !sums) return rc;
   ColumnSums s{};
-  int items = 1;
-  for (int q = 0; q < kVectors; ++q) {
+  int k = 0, sums_y = 0;
+  for (int q = 0; q < kVectors; ++q) {  // the gate's comes last
     if (!out[q]) continue;
     const bool by_item = q == kDGate && a.gate == WUBU_B200_GATE_ITEM;
-    s.part[q] = gr.part + (long long)q * gr.blocks * a.cols;
-    s.out[q] = out[q];
-    s.items[q] = by_item ? (int)a.items : 1;
-    s.n[q] = by_item ? gr.blocks_per_item : (int)gr.blocks;
-    if (s.items[q] > items) items = s.items[q];
+    s.part[k] = gr.part + (long long)q * gr.blocks * a.cols;
+    s.out[k] = out[q];
+    s.n[k] = by_item ? gr.blocks_per_item : (int)gr.blocks;
+    s.count = k++;
+    sums_y += by_item ? (int)a.items : 1;
   }
-  resnorm_sums_kernel<<<dim3((a.cols + kReduceCols - 1) / kReduceCols, items, kVectors), dim3(kReduceCols, kReduceRuns),
-                        0, st>>>(s, a.cols);
+  resnorm_sums_kernel<<<dim3((a.cols + kReduceCols - 1) / kReduceCols, sums_y), dim3(kReduceCols, kReduceRuns), 0, st>>>(
+      s, a.cols);
   return ops_launched("resnorm_sums");
 }
 
