@@ -63,7 +63,8 @@ WB_DEV float act_value(float x, float slope) {
   if (ACT == WUBU_B200_ACT_GELU) {
     float e;
     const float tail = normal_tail(x, e);
-    return fmaf(-fabsf(x), tail, x > 0.f ? x : x * 0.f);  // x Phi(x) = max(x, 0) - |x| Phi(-|x|); NaN stays NaN
+    // x Phi(x) = max(x, 0) - |x| Phi(-|x|), whose second term is 0 from |x| = 64 on; NaN stays NaN
+    return fmaf(-fminf(fabsf(x), 64.f), tail, x > 0.f ? x : x * 0.f);
   }
   if (ACT == WUBU_B200_ACT_SILU) return x * fast_rcp(1.f + fast_ex2(x * -1.4426950408889634f));
   return x;

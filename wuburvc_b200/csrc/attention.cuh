@@ -14,6 +14,8 @@ struct AttnParams {
   int splits;        // forward: parts that the keys are split into, each with an out and an lse of its own
   float* part;       // [splits][B][Hq][Tq][D]
   float* part_lse;   // [splits][B][Hq][Tq]
+  int kv_splits, q_splits;             // backward: parts of the steps of a key tile's and of a query tile's item
+  float *part_dk, *part_dv, *part_dq;  // [splits][B][H][T][D]
   int* err;
   unsigned long long wait_ns;
 };
@@ -21,6 +23,7 @@ struct AttnParams {
 // One item's lengths, and the range of keys that a query sees: query i sits at place i + off.
 struct AttnItem {
   int ql, kl, off;
+  AttnItem() = default;
   WB_DEV AttnItem(const WubuB200Attn& a, int b) {
     ql = a.q_lens ? min(max(__ldg(a.q_lens + b), 0), a.Tq) : a.Tq;
     kl = a.k_lens ? min(max(__ldg(a.k_lens + b), 0), a.Tk) : a.Tk;
@@ -51,10 +54,30 @@ WB_DEV T* at(const WubuB200View& v, int b, int t, int h) {
   return static_cast<T*>(v.data) + b * v.batch + t * v.token + h * v.head;
 }
 
+// The CTAs of a grid no larger than the SMs work through `work` items, heaviest first where that is known:
+// there and back over the CTAs, so that who had the heaviest item of a round has the lightest of the next.
+struct AttnRounds {
+  int work, next, round;
+  WB_DEV AttnRounds(int work_) : work(work_), next(blockIdx.x), round(0) {}
+  WB_DEV bool more() const { return next < work; }
+  WB_DEV void advance() {
+    ++round;
+    next = round * (int)gridDim.x + ((round & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
+  }
+};
+int attn_sms();  // SMs of the current device
+
 int attn_forward(const AttnParams& p, cudaStream_t st);
 long long attn_fwd_bytes(const WubuB200Attn& a);  // the forward's workspace
 long long attn_bwd_bytes(const WubuB200Attn& a);  // the backward's
 int attn_backward(const AttnParams& p, cudaStream_t st);
+
+// bits [lo, hi) of 32
+WB_DEV uint32_t see_bits(int lo, int hi) {
+  const uint32_t below_hi = hi >= 32 ? ~0u : hi <= 0 ? 0u : (1u << hi) - 1u;
+  const uint32_t below_lo = lo >= 32 ? ~0u : lo <= 0 ? 0u : (1u << lo) - 1u;
+  return below_hi & ~below_lo;
+}
 
 // ---- tensor-core tiles ---------------------------------------------------------------------------
 // A tile is 128 tokens of one head in shared memory, as one box of 64 values a row (DP = 64) or two
@@ -150,6 +173,20 @@ WB_DEV void tmem_load(uint32_t taddr, float* v) {  // N columns, a multiple of 3
 #pragma unroll
   for (int g = 0; g < N; g += 32) tmem_use32(v + g);
 }
+WB_DEV void tmem_load16(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < 16; i += 8)
+    asm volatile("" : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]),
+                 "+f"(v[i + 6]), "+f"(v[i + 7]));
+}
 WB_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 WB_DEV void tmem_st32(uint32_t taddr, const uint32_t* r) {
   asm volatile(
@@ -160,6 +197,14 @@ WB_DEV void tmem_st32(uint32_t taddr, const uint32_t* r) {
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
       "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
       "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+WB_DEV void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
       : "memory");
 }
 WB_DEV void mbar_arrive(uint64_t* bar) {
@@ -177,6 +222,27 @@ WB_DEV bool bar_wait(uint64_t* bar, uint32_t parity, int* err, int code, unsigne
       : "memory");
   if (__all_sync(0xffffffffu, done)) return true;
   return mbar_wait_warp(bar, parity, err, code, limit_ns);
+}
+// A warp writes 32 rows x 32 values, a row in each lane (packed pairs w[16]), 64 bytes to a row at a time: through
+// 2 KB of shared memory, 16-byte pieces swizzled by row, then four lanes to a row.  `row` is the first
+// row's address, rows are `stride` elements apart; rows from `rows` and values from `cols` on are left out.
+// (Each lane storing its own row touched 32 lines an instruction and took several thousand cycles a tile.)
+template <typename T>
+WB_DEV void store_rows(uint8_t* stage, const uint32_t* w, T* row, long long stride, int rows, int cols) {
+  const int lane = threadIdx.x & 31;
+  uint4* st = reinterpret_cast<uint4*>(stage);
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    st[lane * 4 + (c ^ (lane >> 1 & 3))] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+  __syncwarp();
+  const int c = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 8 * i + (lane >> 2);
+    const uint4 v = st[r * 4 + (c ^ (r >> 1 & 3))];
+    if (r < rows && c * 8 < cols) *reinterpret_cast<uint4*>(row + r * stride + c * 8) = v;
+  }
+  __syncwarp();
 }
 WB_DEV void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -226,6 +292,27 @@ WB_DEV float max3(float a, float b, float c) {
   return r;
 }
 
+// 2^x of two values on the FMA units, for x up to 120: x = n + f with n a whole number and |f| <= 1/2 (adding and
+// subtracting 1.5 * 2^23 rounds to n), 2^f by a polynomial of degree 4 whose largest relative error is
+// least (2.7e-6 in float32, far below the rounding of P; fitted by reweighted least squares), and n added
+// to the exponent.  Below -125 it returns about 2^-125, which stands for 0.
+WB_DEV uint64_t ex2_poly2(uint64_t x) {
+  float a, b;
+  each(x, a, b);
+  x = two(fmaxf(a, -125.f), fmaxf(b, -125.f));
+  const uint64_t big = two(12582912.f, 12582912.f), t = add2(x, big);
+  const uint64_t f = add2(x, fma2(t, two(-1.f, -1.f), big));  // x - (t - big)
+  uint64_t p = two(0.009570102f, 0.009570102f);
+  p = fma2(p, f, two(0.05591786f, 0.05591786f));
+  p = fma2(p, f, two(0.24024744f, 0.24024744f));
+  p = fma2(p, f, two(0.6931218f, 0.6931218f));
+  p = fma2(p, f, two(0.9999993f, 0.9999993f));
+  float ta, tb;
+  each(t, ta, tb);
+  each(p, a, b);
+  return two(__uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23)),
+             __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23)));
+}
 WB_DEV float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

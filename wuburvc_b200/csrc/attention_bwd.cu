@@ -12,7 +12,8 @@
 // Everything between the products stays in tensor memory.  The first role forms the transposed scores
 // (rows are keys), so that P^T and dS^T are written over them as the A operands of the next products.
 // Eight warps do the exponentials, two to a row quadrant, 64 columns a thread; one warp loads, one
-// issues.  A step's products and its elementwise halves alternate:
+// issues.  A CTA an SM works through the items of both roles, loading the next one's tiles behind the last
+// one's steps; where one item would outlast the rest, its steps are split and float32 parts joined.  A step's products and its elementwise halves alternate:
 //   keys' role:     tensor  dV(n) S(n+1) | dK(n) dP(n+1)      warps  dS(n) | P(n+1)
 //   queries' role:  tensor  dQ(n) dP(n+1) S(n+2)              warps  P(n+1) dS(n+1)
 //
@@ -25,9 +26,13 @@
 namespace wb {
 namespace {
 
-constexpr int kStagesA = 3, kStagesB = 2;  // the keys' role uses two of the first ring
 constexpr int kProducer = 8, kMma = 9, kThreads = 384;
 constexpr float kLog2e = 1.4426950408889634f;
+// Tiles in the ring of Q or K, and of dO or V.  (Of K the second role wants a third, which 128 values a row
+// leave no room for beside the store staging.)
+template <int DP>
+constexpr int kStagesA = DP == 64 ? 3 : 2;
+constexpr int kStagesB = 2;
 
 struct AttnBwdMaps {
   CUtensorMap q, k, v, dout;
@@ -43,8 +48,61 @@ struct BwdShift<f16> {
 };
 
 struct Barriers {
-  uint64_t res_full, a_full[kStagesA], a_empty[kStagesA], b_full[kStagesB], b_empty[kStagesB], s_full[2], dp_full, p_ready,
-      ds_ready, acc_full, mma_done;
+  uint64_t res_full, res_empty, a_full[3], a_empty[3], b_full[kStagesB], b_empty[kStagesB], s_full[2], dp_full, p_ready,
+      ds_ready, acc_full, acc_read, mma_done;
+};
+
+// A work item: 128 keys or 128 queries of one head, and a part of the steps over the other side's tiles.
+struct BwdWork {
+  AttnItem it;
+  bool kv;
+  int b, hk, hq, own0, split;
+  int t0, per_head;      // the other side's first tile and their count, for each head
+  int steps, t, h;       // of this part: steps, and where they start
+  WB_DEV BwdWork(const AttnParams& p, int id, int kv_work) {
+    const WubuB200Attn& a = p.a;
+    kv = id < kv_work;
+    unsigned r = kv ? id : id - kv_work;
+    const unsigned heads = kv ? a.Hkv : a.Hq, splits = kv ? p.kv_splits : p.q_splits;
+    const unsigned u = r / heads;
+    const int head = r - u * heads;
+    r = u / (unsigned)a.B;
+    b = u - r * a.B;
+    it = AttnItem(a, b);
+    split = 0;
+    if (splits > 1) {
+      split = r % splits;
+      r /= splits;
+    }
+    // keys in order (causal: the first have the most queries), queries from the last on
+    own0 = (kv ? (int)r : (a.Tq + kTile - 1) / kTile - 1 - (int)r) * kTile;
+    hk = kv ? head : head / p.group;
+    hq = kv ? head * p.group : head;
+    t0 = per_head = 0;
+    const int last = min(own0 + kTile, kv ? it.kl : it.ql) - 1;
+    if (last >= own0) {
+      const int lo = kv ? it.query_lo(a, own0) : it.key_lo(a, own0), hi = kv ? it.query_hi(a, last) : it.key_hi(a, last);
+      if (hi > lo) {
+        t0 = lo / kTile;
+        per_head = (hi + kTile - 1) / kTile - t0;
+      }
+    }
+    steps = kv ? per_head * p.group : per_head;
+    t = t0;
+    h = kv ? hq : hk;
+    if (splits > 1 && steps) {
+      const int n0 = (int)((long long)steps * split / splits), n1 = (int)((long long)steps * (split + 1) / splits);
+      steps = n1 - n0;
+      h += n0 / per_head;
+      t += n0 % per_head;
+    }
+  }
+  WB_DEV void advance(int& tt, int& hh) const {
+    if (++tt == t0 + per_head) {
+      tt = t0;
+      ++hh;
+    }
+  }
 };
 
 // the power of two that dS is scaled by (fp16), from the bits of the largest squared row norms
@@ -57,73 +115,31 @@ WB_DEV float ds_scale(const AttnParams& p, int b, int hk) {
   return exp2f(fminf(floorf(log2f(16384.f / m)), 100.f));
 }
 
-WB_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}" ::"r"(
-          smem_u32(dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
-}
-
-template <typename T, int DP>
+// SPLIT: in one role at least the steps of an item are split.
+template <typename T, int DP, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
-attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_constant__ AttnParams p, int kv_ctas) {
+attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_constant__ AttnParams p, int kv_work, int work) {
   constexpr int kBoxes = DP / 64;
   constexpr uint32_t kTileBytes = kBoxes * kBox;
+  constexpr int kA = kStagesA<DP>;
   constexpr float kShift = BwdShift<T>::value;
   constexpr int kBf16 = std::is_same<T, bf16>::value;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* res0 = smem;                  // K or Q, for the whole CTA
-  uint8_t* res1 = smem + kTileBytes;     // V or dO
-  uint8_t* ra = smem + 2 * kTileBytes;   // ring of Q or K
-  uint8_t* rb = ra + kStagesA * kTileBytes;  // ring of dO or V
+  uint8_t* res0 = smem;                    // K or Q, for a whole item
+  uint8_t* res1 = smem + kTileBytes;       // V or dO
+  uint8_t* ra = smem + 2 * kTileBytes;     // ring of Q or K
+  uint8_t* rb = ra + kA * kTileBytes;      // ring of dO or V
+  uint8_t* stage = rb + kStagesB * kTileBytes;  // 2 KB a warp
   __shared__ Barriers bar;
   __shared__ uint32_t tmem_slot;
-  // keys' role: the log-sum-exp and D of a step's 128 queries, two steps, in the first ring's third tile
-  float* rows = reinterpret_cast<float*>(ra + 2 * kTileBytes);
 
   const WubuB200Attn& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool kv = (int)blockIdx.x < kv_ctas;
-  // this CTA's tile: keys in order (causal: the first have the most queries), queries from the last on
-  int tile, hq, hk, b, t0 = 0, t1 = 0, heads;
-  {
-    const int heads_all = (kv ? a.Hkv : a.Hq) * a.B;
-    const int id = kv ? (int)blockIdx.x : (int)blockIdx.x - kv_ctas;
-    const int r = id / heads_all, hb = id - r * heads_all;
-    const int h = hb % (kv ? a.Hkv : a.Hq);
-    b = hb / (kv ? a.Hkv : a.Hq);
-    tile = kv ? r : (a.Tq + kTile - 1) / kTile - 1 - r;
-    hk = kv ? h : h / p.group;
-    hq = kv ? h * p.group : h;
-    heads = kv ? p.group : 1;
-  }
-  const AttnItem it(a, b);
-  const int own0 = tile * kTile;
-  {  // the other side's tiles [t0, t1) that any of this tile's rows meets
-    const int last = min(own0 + kTile, kv ? it.kl : it.ql) - 1;
-    if (last >= own0) {
-      const int lo = kv ? it.query_lo(a, own0) : it.key_lo(a, own0), hi = kv ? it.query_hi(a, last) : it.key_hi(a, last);
-      if (hi > lo) {
-        t0 = lo / kTile;
-        t1 = (hi + kTile - 1) / kTile;
-      }
-    }
-  }
-  const int per_head = t1 - t0, steps = per_head * heads;
-  // slot and phase of step n in the rings
-  const int na = kv ? 2 : kStagesA;
-  auto slot_a = [&](int n) { return kv ? n & 1 : n % kStagesA; };
-  auto phase_a = [&](int n) { return (uint32_t)(kv ? n >> 1 : n / kStagesA) & 1u; };
-  auto slot_b = [&](int n) { return n % kStagesB; };
-  auto phase_b = [&](int n) { return (uint32_t)(n / kStagesB) & 1u; };
-
   if (threadIdx.x == 0) {
     mbar_init(&bar.res_full, 1);
-    for (int i = 0; i < kStagesA; ++i) {
+    mbar_init(&bar.res_empty, 1);
+    for (int i = 0; i < kA; ++i) {
       mbar_init(&bar.a_full[i], 1);
       mbar_init(&bar.a_empty[i], 1);
     }
@@ -137,6 +153,7 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
     mbar_init(&bar.p_ready, 8);
     mbar_init(&bar.ds_ready, 8);
     mbar_init(&bar.acc_full, 1);
+    mbar_init(&bar.acc_read, 8);
     mbar_init(&bar.mma_done, 1);
     fence_barrier_init();
   }
@@ -144,43 +161,43 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  // keys' role: S at 0, dP at 128, dV at 256, dK at 384; queries' role: S at 0 and 128, dP at 256, dQ at 384
-  const uint32_t tDP = tmem + (kv ? 128 : 256), tAcc0 = tmem + 256, tAcc1 = tmem + 384;
+  // columns: S at 0 (queries' role: every second step's at 256), dP at 128, dV at 256, dK or dQ at 384
+  const uint32_t tDP = tmem + 128, tAcc0 = tmem + 256, tAcc1 = tmem + 384;
 
   if (warp >= kProducer) {
     regs_dec<72>();
     if (warp == kProducer) {
       bool ok = true;
       FillTrack fr, fa, fb;
-      if (steps > 0) {
-        fr.fill(0, 0);
-        mbar_expect_tx_warp(&bar.res_full, 2 * kTileBytes);
-        load_tile(res0, kv ? &maps.k : &maps.q, &bar.res_full, own0, kv ? hk : hq, b, kBoxes);
-        load_tile(res1, kv ? &maps.v : &maps.dout, &bar.res_full, own0, kv ? hk : hq, b, kBoxes);
-      }
-      int t = t0, h = kv ? hq : hk;
-      for (int n = 0; n < steps; ++n) {
-        const int sa = slot_a(n), sb = slot_b(n);
-        if (ok && n >= na) ok = bar_wait(&bar.a_empty[sa], phase_a(n) ^ 1u, p.err, ERR_WAIT_EMPTY, p.wait_ns);
+      int n = 0, items = 0;  // steps and items (with steps) so far
+      for (AttnRounds r(work); r.more(); r.advance()) {
+        const BwdWork k(p, r.next, kv_work);
+        if (k.steps == 0) continue;
+        if (ok && items) ok = bar_wait(&bar.res_empty, (items - 1) & 1, p.err, ERR_WAIT_EMPTY, p.wait_ns);
         if (ok) {
-          fa.fill(sa, phase_a(n));
-          mbar_expect_tx_warp(&bar.a_full[sa], kTileBytes + (kv ? 2 * kTile * 4 : 0));
-          load_tile(ra + sa * kTileBytes, kv ? &maps.q : &maps.k, &bar.a_full[sa], t * kTile, h, b, kBoxes);
-          if (kv) {
-            const long long r = ((long long)b * a.Hq + h) * p.t_pad + t * kTile;
-            bulk_load(rows + sa * 2 * kTile, p.lse2 + r, kTile * 4, &bar.a_full[sa]);
-            bulk_load(rows + sa * 2 * kTile + kTile, p.delta + r, kTile * 4, &bar.a_full[sa]);
+          fr.fill(0, items);
+          mbar_expect_tx_warp(&bar.res_full, 2 * kTileBytes);
+          load_tile(res0, k.kv ? &maps.k : &maps.q, &bar.res_full, k.own0, k.kv ? k.hk : k.hq, k.b, kBoxes);
+          load_tile(res1, k.kv ? &maps.v : &maps.dout, &bar.res_full, k.own0, k.kv ? k.hk : k.hq, k.b, kBoxes);
+        }
+        ++items;
+        int t = k.t, h = k.h;
+        for (int i = 0; i < k.steps; ++i, ++n) {
+          const int sa = n % kA, sb = n % kStagesB;
+          const uint32_t pa = (n / kA) & 1, pb = (n / kStagesB) & 1;
+          if (ok && n >= kA) ok = bar_wait(&bar.a_empty[sa], pa ^ 1u, p.err, ERR_WAIT_EMPTY, p.wait_ns);
+          if (ok) {
+            fa.fill(sa, pa);
+            mbar_expect_tx_warp(&bar.a_full[sa], kTileBytes);
+            load_tile(ra + sa * kTileBytes, k.kv ? &maps.q : &maps.k, &bar.a_full[sa], t * kTile, h, k.b, kBoxes);
           }
-        }
-        if (ok && n >= kStagesB) ok = bar_wait(&bar.b_empty[sb], phase_b(n) ^ 1u, p.err, ERR_WAIT_EMPTY, p.wait_ns);
-        if (ok) {
-          fb.fill(sb, phase_b(n));
-          mbar_expect_tx_warp(&bar.b_full[sb], kTileBytes);
-          load_tile(rb + sb * kTileBytes, kv ? &maps.dout : &maps.v, &bar.b_full[sb], t * kTile, h, b, kBoxes);
-        }
-        if (++t == t1) {
-          t = t0;
-          ++h;
+          if (ok && n >= kStagesB) ok = bar_wait(&bar.b_empty[sb], pb ^ 1u, p.err, ERR_WAIT_EMPTY, p.wait_ns);
+          if (ok) {
+            fb.fill(sb, pb);
+            mbar_expect_tx_warp(&bar.b_full[sb], kTileBytes);
+            load_tile(rb + sb * kTileBytes, k.kv ? &maps.dout : &maps.v, &bar.b_full[sb], t * kTile, h, k.b, kBoxes);
+          }
+          k.advance(t, h);
         }
       }
       fr.drain(&bar.res_full, p.err, p.wait_ns);  // no copy of this CTA may land after it exits
@@ -191,65 +208,79 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
       const uint32_t id_o = make_idesc(128, (a.D + 15) / 16 * 16, 0, 1, kBf16);
       const int ksteps = (a.D + 15) / 16;
       const uint64_t dr0 = desc_k(res0), dr1 = desc_k(res1);
-      bool ok = steps > 0 ? bar_wait(&bar.res_full, 0, p.err, ERR_WAIT_FULL, p.wait_ns) : true;
-      // rows of step n's tiles beyond the item's length
-      auto valid = [&](int n) { return (kv ? it.ql : it.kl) - (t0 + n % per_head) * kTile; };
-      auto wait_a = [&](int n) {
-        const int st = slot_a(n);
-        if (ok) ok = bar_wait(&bar.a_full[st], phase_a(n), p.err, ERR_WAIT_FULL, p.wait_ns);
-        if (ok && valid(n) < kTile) zero_rows(ra + st * kTileBytes, max(valid(n), 0), kBoxes);
-      };
-      auto wait_b = [&](int n) {
-        const int st = slot_b(n);
-        if (ok) ok = bar_wait(&bar.b_full[st], phase_b(n), p.err, ERR_WAIT_FULL, p.wait_ns);
-        if (ok && valid(n) < kTile) zero_rows(rb + st * kTileBytes, max(valid(n), 0), kBoxes);
-      };
-      auto issue_s = [&](int n) {
-        wait_a(n);
-        const int buf = kv ? 0 : n & 1;
-        if (ok) {
-          mma_values<DP>(tmem + 128 * buf, dr0, desc_k(ra + slot_a(n) * kTileBytes), id_s, ksteps);
-          umma_commit_warp(&bar.s_full[buf]);
-        }
-      };
-      auto issue_dp = [&](int n) {
-        wait_b(n);
-        if (ok) {
-          mma_values<DP>(tDP, dr1, desc_k(rb + slot_b(n) * kTileBytes), id_s, ksteps);
-          umma_commit_warp(&bar.dp_full);
-          if (!kv) umma_commit_warp(&bar.b_empty[slot_b(n)]);  // nothing else reads V
-        }
-      };
-      // acc += (A in tensor memory, 128 x 128, its halves 64 columns apart) x tile
-      auto issue_acc = [&](uint32_t acc, uint32_t src, const uint8_t* tile_, int n) {
-        const uint64_t d = desc_mn(tile_);
-        mma4_ts(acc, src, d, id_o, n > 0);
-        mma4_ts(acc, src + 64, d + (4 * 2048u >> 4), id_o, 1);
-      };
-      if (steps > 0) {
+      bool ok = true;
+      int n0 = 0, items = 0, p_count = 0;
+      int all = 0;  // items so far, those without steps too
+      for (AttnRounds r(work); r.more(); r.advance(), ++all) {
+        const BwdWork k(p, r.next, kv_work);
+        if (k.steps == 0) continue;
+        const bool kv = k.kv;
+        if (ok) ok = bar_wait(&bar.res_full, items & 1, p.err, ERR_WAIT_FULL, p.wait_ns);
+        ++items;
+        int ta = k.t, tb = k.t, unused = 0;  // tiles of the next S and dP
+        // step n's tile in a ring, its rows beyond the item's length cleared
+        auto clear = [&](uint8_t* tile, int tt) {
+          const int valid = (kv ? k.it.ql : k.it.kl) - tt * kTile;
+          if (ok && valid < kTile) zero_rows(tile, max(valid, 0), kBoxes);
+        };
+        auto issue_s = [&](int i) {
+          const int n = n0 + i, sa = n % kA, buf = kv ? 0 : i & 1;
+          if (ok) ok = bar_wait(&bar.a_full[sa], (n / kA) & 1, p.err, ERR_WAIT_FULL, p.wait_ns);
+          clear(ra + sa * kTileBytes, ta);
+          k.advance(ta, unused);
+          if (ok) {
+            mma_values<DP>(tmem + 256 * buf, dr0, desc_k(ra + sa * kTileBytes), id_s, ksteps);
+            umma_commit_warp(&bar.s_full[buf]);
+          }
+        };
+        auto issue_dp = [&](int i) {
+          const int n = n0 + i, sb = n % kStagesB;
+          if (ok) ok = bar_wait(&bar.b_full[sb], (n / kStagesB) & 1, p.err, ERR_WAIT_FULL, p.wait_ns);
+          clear(rb + sb * kTileBytes, tb);
+          k.advance(tb, unused);
+          if (ok) {
+            mma_values<DP>(tDP, dr1, desc_k(rb + sb * kTileBytes), id_s, ksteps);
+            umma_commit_warp(&bar.dp_full);
+            if (!kv) umma_commit_warp(&bar.b_empty[sb]);  // nothing else reads V
+            if (i == k.steps - 1) umma_commit_warp(&bar.res_empty);
+          }
+        };
+        // acc += (A in tensor memory, 128 x 128, its halves 64 columns apart) x tile
+        auto issue_acc = [&](uint32_t acc, uint32_t src, const uint8_t* tile, int i) {
+          const uint64_t d = desc_mn(tile);
+          mma4_ts(acc, src, d, id_o, i > 0);
+          mma4_ts(acc, src + 64, d + (4 * 2048u >> 4), id_o, 1);
+        };
         issue_s(0);
         issue_dp(0);
-        if (!kv && steps > 1) issue_s(1);
-      }
-      for (int n = 0; n < steps; ++n) {
-        const uint32_t ph = n & 1;
-        if (kv) {
-          if (ok) ok = bar_wait(&bar.p_ready, ph, p.err, ERR_WAIT_ACC, p.wait_ns);
+        if (!kv && k.steps > 1) {
+          // the second buffer of S may still be the last item's dV
+          if (ok && all) ok = bar_wait(&bar.acc_read, (all - 1) & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
           tc_fence_after();
-          if (ok) issue_acc(tAcc0, tmem, rb + slot_b(n) * kTileBytes, n);
-          if (n + 1 < steps) issue_s(n + 1);
+          issue_s(1);
         }
-        if (ok) ok = bar_wait(&bar.ds_ready, ph, p.err, ERR_WAIT_ACC, p.wait_ns);
-        tc_fence_after();
-        if (ok) {
-          issue_acc(tAcc1, tDP, ra + slot_a(n) * kTileBytes, n);
-          umma_commit_warp(&bar.a_empty[slot_a(n)]);
-          if (kv) umma_commit_warp(&bar.b_empty[slot_b(n)]);
+        for (int i = 0; i < k.steps; ++i) {
+          const int n = n0 + i, sa = n % kA, sb = n % kStagesB;
+          if (kv) {
+            if (ok) ok = bar_wait(&bar.p_ready, p_count & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
+            ++p_count;
+            tc_fence_after();
+            if (ok) issue_acc(tAcc0, tmem, rb + sb * kTileBytes, i);
+            if (i + 1 < k.steps) issue_s(i + 1);
+          }
+          if (ok) ok = bar_wait(&bar.ds_ready, n & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
+          tc_fence_after();
+          if (ok) {
+            issue_acc(tAcc1, tDP, ra + sa * kTileBytes, i);
+            umma_commit_warp(&bar.a_empty[sa]);
+            if (kv) umma_commit_warp(&bar.b_empty[sb]);
+            if (i == k.steps - 1) umma_commit_warp(&bar.acc_full);
+          }
+          if (i + 1 < k.steps) issue_dp(i + 1);
+          if (!kv && i + 2 < k.steps) issue_s(i + 2);
         }
-        if (n + 1 < steps) issue_dp(n + 1);
-        if (!kv && n + 2 < steps) issue_s(n + 2);
+        n0 += k.steps;
       }
-      if (ok) umma_commit_warp(&bar.acc_full);
       // every MMA this warp issued has completed before TMEM is released (also after a timed-out wait)
       umma_commit_warp(&bar.mma_done);
       bar_wait(&bar.mma_done, 0, p.err, ERR_WAIT_ACC, p.wait_ns);
@@ -258,112 +289,153 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
     regs_inc<216>();
     const int half = warp >> 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const int row = own0 + (warp & 3) * 32 + lane;  // a key or a query
-    const float c = a.scale * kLog2e;
-    const float f = ds_scale<T>(p, b, hk) * exp2f(-kShift);  // on P 2^shift (dP - D)
-    const int lo = kv ? it.query_lo(a, row) : it.key_lo(a, row), hi = kv ? it.query_hi(a, row) : it.key_hi(a, row);
-    // tiles that all of this tile's live rows meet whole need no mask
-    const int last = min(own0 + kTile, kv ? it.kl : it.ql) - 1;
-    const int all_lo = last >= own0 ? (kv ? it.query_lo(a, last) : it.key_lo(a, last)) : 0;
-    const int all_hi = kv ? it.query_hi(a, own0) : it.key_hi(a, own0);
-    float l2 = 0.f, delta = 0.f;
-    if (!kv && steps > 0) {
-      const long long r = ((long long)b * a.Hq + hq) * p.t_pad + row;
-      l2 = p.lse2[r];
-      delta = p.delta[r];
-    }
     const uint32_t DPc = tDP + lanes + 64 * half;
+    const float c = a.scale * kLog2e;
     bool ok = true;
-    for (int n = 0; n < steps; ++n) {
-      const int st = slot_a(n), col0 = (t0 + n % per_head) * kTile + 64 * half;
-      const uint32_t S = tmem + (kv ? 0 : 128 * (n & 1)) + lanes + 64 * half;
-      if (kv && ok) ok = bar_wait(&bar.a_full[st], phase_a(n), p.err, ERR_WAIT_FULL, p.wait_ns);
-      if (ok)
-        ok = kv ? bar_wait(&bar.s_full[0], n & 1, p.err, ERR_WAIT_ACC, p.wait_ns)
-                : bar_wait(&bar.s_full[n & 1], (n >> 1) & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
-      if (!ok) continue;
-      tc_fence_after();
-      float x[64];
-      tmem_load<64>(S, x);
-      if (kv) {
-        const float4* ls = reinterpret_cast<const float4*>(rows + st * 2 * kTile + 64 * half);
+    int n0 = 0, items = 0;         // steps and items (with steps) so far
+    uint32_t s_phase[2] = {0, 0};  // of the two buffers of S
+    griddep_wait();                // the row sums and log-sum-exps come from the kernel before
+    for (AttnRounds r(work); r.more(); r.advance()) {
+      const BwdWork k(p, r.next, kv_work);
+      const bool kv = k.kv;
+      const AttnItem it = k.it;
+      const int row = k.own0 + (warp & 3) * 32 + lane;  // a key or a query
+      const int lo = kv ? it.query_lo(a, row) : it.key_lo(a, row), hi = kv ? it.query_hi(a, row) : it.key_hi(a, row);
+      // tiles that all of this tile's live rows meet whole need no mask
+      const int last = min(k.own0 + kTile, kv ? it.kl : it.ql) - 1;
+      const int all_lo = last >= k.own0 ? (kv ? it.query_lo(a, last) : it.key_lo(a, last)) : 0;
+      const int all_hi = kv ? it.query_hi(a, k.own0) : it.key_hi(a, k.own0);
+      const float f = kBf16 ? 1.f : ds_scale<T>(p, k.b, k.hk) * exp2f(-kShift);  // on P 2^shift (dP - D)
+      float l2 = 0.f, delta = 0.f;
+      if (!kv && k.steps > 0) {
+        const long long q = ((long long)k.b * a.Hq + k.hq) * p.t_pad + row;
+        l2 = p.lse2[q];
+        delta = p.delta[q];
+      }
+      int t = k.t, h = k.h;
+      for (int i = 0; i < k.steps; ++i) {
+        const int col0 = t * kTile + 64 * half, buf = kv ? 0 : i & 1;
+        const uint32_t S = tmem + 256 * buf + lanes + 64 * half;
+        const long long q0 = ((long long)k.b * a.Hq + h) * p.t_pad + col0;  // keys' role: the step's queries
+        const bool masked = t * kTile < all_lo || t * kTile + kTile > all_hi;
+        k.advance(t, h);
+        float rows[64];
+        if (kv) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float4 v = ls[k];
-          x[4 * k] = ex2(fmaf(x[4 * k], c, kShift - v.x));
-          x[4 * k + 1] = ex2(fmaf(x[4 * k + 1], c, kShift - v.y));
-          x[4 * k + 2] = ex2(fmaf(x[4 * k + 2], c, kShift - v.z));
-          x[4 * k + 3] = ex2(fmaf(x[4 * k + 3], c, kShift - v.w));
+          for (int e = 0; e < 16; ++e) *reinterpret_cast<float4*>(rows + 4 * e) = *reinterpret_cast<const float4*>(p.lse2 + q0 + 4 * e);
         }
-      } else {
+        if (ok) ok = bar_wait(&bar.s_full[buf], buf ? s_phase[1] : s_phase[0], p.err, ERR_WAIT_ACC, p.wait_ns);
+        if (buf) s_phase[1] ^= 1u;
+        else s_phase[0] ^= 1u;
+        if (!ok) continue;
+        tc_fence_after();
+        float x[64];
+        tmem_load<64>(S, x);
+        if (kv) {
 #pragma unroll
-        for (int k = 0; k < 64; ++k) x[k] = ex2(fmaf(x[k], c, kShift - l2));
-      }
-      if (col0 - 64 * half < all_lo || col0 - 64 * half + kTile > all_hi) {
-        const int r0 = lo - col0, r1 = hi - col0;
+          for (int e = 0; e < 64; ++e) x[e] = ex2(fmaf(x[e], c, kShift - rows[e]));
+        } else {
+          const uint64_t cc = two(c, c), ll = two(kShift - l2, kShift - l2);
 #pragma unroll
-        for (int k = 0; k < 64; ++k) x[k] = k >= r0 && k < r1 ? x[k] : 0.f;
-      }
-      uint32_t w[32];
-      if (kv) {
+          for (int e = 0; e < 64; e += 2) each(fma2(two(x[e], x[e + 1]), cc, ll), x[e], x[e + 1]);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) w[k] = pack2(x[2 * k], x[2 * k + 1], T());
-        tmem_st32(S, w);
+          for (int e = 0; e < 64; ++e) x[e] = ex2(x[e]);
+        }
+        if (masked) {
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const uint32_t see = see_bits(lo - col0 - 32 * g, hi - col0 - 32 * g);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[32 * g + e] = see >> e & 1 ? x[32 * g + e] : 0.f;
+          }
+        }
+        if (kv) {
+          uint32_t w[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) w[e] = pack2(x[2 * e], x[2 * e + 1], T());
+          tmem_st32(S, w);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar.p_ready);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) *reinterpret_cast<float4*>(rows + 4 * e) = *reinterpret_cast<const float4*>(p.delta + q0 + 4 * e);
+        }
+        ok = bar_wait(&bar.dp_full, (n0 + i) & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
+        if (!ok) continue;
+        tc_fence_after();
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          float y[32];
+          uint32_t w[16];
+          tmem_load<32>(DPc + 32 * g, y);
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float* d = rows + 32 * g + e;
+            uint64_t v = add2(two(y[e], y[e + 1]), kv ? two(-d[0], -d[1]) : two(-delta, -delta));
+            v = mul2(v, two(x[32 * g + e], x[32 * g + e + 1]));
+            if (!kBf16) v = mul2(v, two(f, f));
+            each(v, y[e], y[e + 1]);
+            w[e / 2] = pack2(y[e], y[e + 1], T());
+          }
+          tmem_st16(DPc + 16 * g, w);  // over columns that have been read
+        }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.p_ready);
+        if (lane == 0) mbar_arrive(&bar.ds_ready);
       }
-      ok = bar_wait(&bar.dp_full, n & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
-      if (!ok) continue;
-      tc_fence_after();
-      float y[64];
-      tmem_load<64>(DPc, y);
-      const float4* ds = reinterpret_cast<const float4*>(rows + st * 2 * kTile + kTile + 64 * half);
-#pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        float4 v = make_float4(delta, delta, delta, delta);
-        if (kv) v = ds[k];
-        float g[4] = {y[4 * k] - v.x, y[4 * k + 1] - v.y, y[4 * k + 2] - v.z, y[4 * k + 3] - v.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          g[e] *= x[4 * k + e];
-          if (!kBf16) g[e] *= f;
-        }
-        w[2 * k] = pack2(g[0], g[1], T());
-        w[2 * k + 1] = pack2(g[2], g[3], T());
+      n0 += k.steps;
+      if (k.steps > 0) {
+        if (ok) ok = bar_wait(&bar.acc_full, items & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
+        ++items;
+        tc_fence_after();
       }
-      tmem_st32(DPc, w);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.ds_ready);
-    }
-    if (steps > 0 && ok) ok = bar_wait(&bar.acc_full, 0, p.err, ERR_WAIT_ACC, p.wait_ns);
-    tc_fence_after();
-    // the accumulators, half of the columns to each warpgroup
-    const bool live = hi > lo && steps > 0 && ok;
-    const float ds_out = a.scale / (kBf16 ? 1.f : f * exp2f(kShift));
-    const float p_out = exp2f(-kShift);
-#pragma unroll
-    for (int g = 0; g < DP / 64; ++g) {
-      const int d0 = half * (DP / 2) + 32 * g;
+      // the accumulators, half of the columns to each warpgroup
+      const bool live = hi > lo && k.steps > 0 && ok;
+      const float ds_out = a.scale / (kBf16 ? 1.f : f * exp2f(kShift)), p_out = exp2f(-kShift);
+      const int d0 = DP / 2 * half;
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
         if (!kv && which == 0) continue;
-        float o[32];
-        if (steps > 0) tmem_load<32>((which ? tAcc1 : tAcc0) + lanes + d0, o);
         const float sc = which ? ds_out : p_out;
+        auto values = [&](int d, float* o) {  // 32 of the row's results, from d0 + d
+          if (k.steps > 0) tmem_load<32>((which ? tAcc1 : tAcc0) + lanes + d0 + d, o);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) o[k] = live ? o[k] * sc : 0.f;
-        if (row >= (kv ? a.Tk : a.Tq)) continue;
-        T* out = kv ? (which ? at<T>(a.dk, b, row, hk) : at<T>(a.dv, b, row, hk)) : at<T>(a.dq, b, row, hq);
+          for (int e = 0; e < 32; ++e) o[e] = live ? o[e] * sc : 0.f;
+        };
+        if (SPLIT && (kv ? p.kv_splits : p.q_splits) > 1) {
+          const long long T_ = kv ? a.Tk : a.Tq, H = kv ? a.Hkv : a.Hq, all = a.B * H * T_ * a.D;
+          float* part = (!kv ? p.part_dq : which ? p.part_dk : p.part_dv) + k.split * all +
+                        (((long long)k.b * H + (kv ? k.hk : k.hq)) * T_ + row) * a.D + d0;
 #pragma unroll
-        for (int k = 0; k < 32; k += 8)
-          if (d0 + k < a.D) store8(out + d0 + k, o + k);
+          for (int d = 0; d < DP / 2; d += 32) {
+            float o[32];
+            values(d, o);
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+              if (row < T_ && d0 + d + e < a.D) store8(part + d + e, o + e);
+            __syncwarp();
+          }
+        } else {
+          const int r0 = k.own0 + (warp & 3) * 32;
+          const WubuB200View& view = !kv ? a.dq : which ? a.dk : a.dv;
+          T* out = at<T>(view, k.b, r0, kv ? k.hk : k.hq) + d0;
+#pragma unroll
+          for (int d = 0; d < DP / 2; d += 32) {
+            float o[32];
+            values(d, o);
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w[e] = pack2(o[2 * e], o[2 * e + 1], T());
+            store_rows(stage + warp * 2048, w, out + d, view.token, (kv ? a.Tk : a.Tq) - r0, a.D - d0 - d);
+          }
+        }
       }
+      tc_fence_before();  // the accumulators are read before the next item's products may be issued
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.acc_read);
     }
-    tc_fence_before();
   }
   __syncthreads();
   tc_fence_after();
@@ -382,27 +454,27 @@ WB_DEV float dot8(const T* x, const T* y) {
 
 // delta = rowsum(dO * O) and the log-sum-exp in units of log 2, padded to whole tiles with what gives
 // probability 0; for fp16 also the largest squared norms of dO's and V's rows (an integer maximum over
-// the bits of non-negative floats: its order does not matter).  16 threads a row.
-template <typename T>
+// the bits of non-negative floats: its order does not matter).  N threads a row, 8 values each.
+template <typename T, int N>
 __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnParams p) {
   const WubuB200Attn& a = p.a;
-  const int t = threadIdx.x & 15, i = blockIdx.x * 16 + threadIdx.x / 16, h = blockIdx.y, b = blockIdx.z;
+  const int t = threadIdx.x % N, i = blockIdx.x * (256 / N) + threadIdx.x / N, h = blockIdx.y, b = blockIdx.z;
   const AttnItem it(a, b);
+  constexpr bool kNorms = std::is_same<T, f16>::value;
   float d = 0.f, g = 0.f, v = 0.f;
   if (i < it.ql && t * 8 < a.D) {
     const T* x = at<T>(a.dout, b, i, h) + t * 8;
     d = dot8(x, at<T>(a.out, b, i, h) + t * 8);
-    if (std::is_same<T, f16>::value) g = dot8(x, x);
+    if (kNorms) g = dot8(x, x);
   }
-  const bool keys = std::is_same<T, f16>::value && h % p.group == 0;
-  if (keys && i < it.kl && t * 8 < a.D) {
+  if (kNorms && h % p.group == 0 && i < it.kl && t * 8 < a.D) {
     const T* x = at<T>(a.v, b, i, h / p.group) + t * 8;
     v = dot8(x, x);
   }
 #pragma unroll
-  for (int m = 1; m < 16; m <<= 1) {
+  for (int m = 1; m < N; m <<= 1) {
     d += __shfl_xor_sync(0xffffffffu, d, m);
-    if (std::is_same<T, f16>::value) {
+    if (kNorms) {
       g += __shfl_xor_sync(0xffffffffu, g, m);
       v += __shfl_xor_sync(0xffffffffu, v, m);
     }
@@ -413,7 +485,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnParams p) {
     p.delta[r] = d;
     p.lse2[r] = l == -INFINITY ? INFINITY : l;
   }
-  if (std::is_same<T, f16>::value) {
+  if (kNorms) {
     const int n = a.B * a.Hkv, at_ = b * a.Hkv + h / p.group;
     const uint32_t gm = __reduce_max_sync(0xffffffffu, __float_as_uint(g));
     const uint32_t vm = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
@@ -424,48 +496,118 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnParams p) {
   }
 }
 
+// A gradient from the float32 sums of its parts, in order; 8 values a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_join_kernel(const float* part, int splits, WubuB200View out, int B, int H,
+                                                        int tokens, int D) {
+  griddep_wait();
+  const long long all = (long long)B * H * tokens * D, at8 = ((long long)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (at8 >= all) return;
+  float o[8] = {};
+  for (int s = 0; s < splits; ++s) {
+    const float4 u = *reinterpret_cast<const float4*>(part + s * all + at8), v = *reinterpret_cast<const float4*>(part + s * all + at8 + 4);
+    o[0] += u.x; o[1] += u.y; o[2] += u.z; o[3] += u.w;
+    o[4] += v.x; o[5] += v.y; o[6] += v.z; o[7] += v.w;
+  }
+  const int d = (int)(at8 % D);
+  const long long r = at8 / D;
+  const int i = (int)(r % tokens), h = (int)(r / tokens % H), b = (int)(r / tokens / H);
+  store8(at<T>(out, b, i, h) + d, o);
+}
+
+long long tiles_of(int T) { return (T + kTile - 1) / kTile; }
+
+// Into how many parts the steps of a key tile's and of a query tile's item are split.  The grid is as long as its
+// longest item: where that (4 products a step in the keys' role, 3 in the other) is longer than an even
+// share of all the work, which happens with few heads or many that share a key head, it is cut to about
+// that share.  (4 x 4001 tokens causal, 16 query heads on 4: parts of 2.)  Causal order halves the work
+// but not the longest item.
+void bwd_splits(const WubuB200Attn& a, int sms, int& kv, int& q) {
+  const long long nq = tiles_of(a.Tq), nk = tiles_of(a.Tk), group = a.Hkv ? a.Hq / a.Hkv : 1;
+  const long long kv_item = 4 * nq * group, q_item = 3 * nk;
+  const long long share = (kv_item * nk * a.Hkv + q_item * nq * a.Hq) * a.B / (a.causal ? 2 : 1) / (sms > 0 ? sms : 1) + 1;
+  auto parts = [&](long long item, long long steps) {
+    long long s = (item + share - 1) / share;
+    if (s > (steps + 1) / 2) s = (steps + 1) / 2;  // two steps at least, for the prologue's sake
+    return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
+  };
+  kv = parts(kv_item, nq * group);
+  q = parts(q_item, nk);
+}
+
 template <typename T, int DP>
-int launch_bwd(const AttnBwdMaps& maps, const AttnParams& p, cudaStream_t st) {
+int launch_bwd(const AttnBwdMaps& maps, const AttnParams& p, int sms, cudaStream_t st) {
   const WubuB200Attn& a = p.a;
-  constexpr int smem = (2 + kStagesA + kStagesB) * (DP / 64) * (int)kBox + 1024;
-  static std::atomic<uint64_t> devices{0};
-  if (!ops_smem_limit((const void*)attn_bwd_tc_kernel<T, DP>, smem, devices)) return WUBU_B200_ERR_CUDA;
+  constexpr int smem = (2 + kStagesA<DP> + kStagesB) * (DP / 64) * (int)kBox + 8 * 2048 + 1024;
+  static std::atomic<uint64_t> devices[2];
+  auto* kernel = p.kv_splits > 1 || p.q_splits > 1 ? attn_bwd_tc_kernel<T, DP, true> : attn_bwd_tc_kernel<T, DP, false>;
+  if (!ops_smem_limit((const void*)attn_bwd_tc_kernel<T, DP, true>, smem, devices[0]) ||
+      !ops_smem_limit((const void*)attn_bwd_tc_kernel<T, DP, false>, smem, devices[1]))
+    return WUBU_B200_ERR_CUDA;
   if (std::is_same<T, f16>::value &&
       cudaMemsetAsync(p.norm_bits, 0, 2ull * a.B * a.Hkv * sizeof(unsigned), st) != cudaSuccess)
     return WUBU_B200_ERR_CUDA;
   const int rows = std::is_same<T, f16>::value && a.Tk > p.t_pad ? a.Tk : p.t_pad;
-  if (rows) attn_delta_kernel<T><<<dim3((rows + 15) / 16, a.Hq, a.B), 256, 0, st>>>(p);
+  constexpr int kRows = 256 / (DP / 8);
+  if (rows) attn_delta_kernel<T, DP / 8><<<dim3((rows + kRows - 1) / kRows, a.Hq, a.B), 256, 0, st>>>(p);
   int rc = ops_launched("attn_backward rows");
   if (rc != WUBU_B200_OK) return rc;
-  const long long kv = (long long)((a.Tk + kTile - 1) / kTile) * a.Hkv * a.B;
-  const long long qs = (long long)((a.Tq + kTile - 1) / kTile) * a.Hq * a.B;
-  if (kv + qs > 0x7FFFFFFFll) return WUBU_B200_ERR_SHAPE;
-  attn_bwd_tc_kernel<T, DP><<<(unsigned)(kv + qs), kThreads, smem, st>>>(maps, p, (int)kv);
-  return ops_launched("attn_backward");
+  const long long kv = tiles_of(a.Tk) * a.Hkv * a.B * p.kv_splits, qs = tiles_of(a.Tq) * a.Hq * a.B * p.q_splits;
+  if (kv + qs > 0x3FFFFFFF) return WUBU_B200_ERR_SHAPE;
+  const int work = (int)(kv + qs);
+  rc = ops_launch_after(kernel, dim3(work < sms ? work : sms), dim3(kThreads), smem, st,
+                        "attn_backward", maps, p, (int)kv, work);
+  auto join = [&](const float* part, int splits, const WubuB200View& out, int H, int tokens) {
+    const long long n8 = (long long)a.B * H * tokens * a.D / 8;
+    if (rc == WUBU_B200_OK && splits > 1 && n8)
+      rc = ops_launch_after(attn_join_kernel<T>, dim3((unsigned)((n8 + 255) / 256)), dim3(256), 0, st, "attn_backward join",
+                            part, splits, out, a.B, H, tokens, a.D);
+  };
+  join(p.part_dk, p.kv_splits, a.dk, a.Hkv, a.Tk);
+  join(p.part_dv, p.kv_splits, a.dv, a.Hkv, a.Tk);
+  join(p.part_dq, p.q_splits, a.dq, a.Hq, a.Tq);
+  return rc;
+}
+
+// The workspace: delta, lse2, norm bits (to a multiple of 16 bytes), then the parts of dk, dv and dq.
+long long bwd_layout(const WubuB200Attn& a, AttnParams* p) {
+  int kv = 1, q = 1;
+  bwd_splits(a, attn_sms(), kv, q);
+  const long long rows = (long long)a.B * a.Hq * tiles_of(a.Tq) * kTile, bits = (2ll * a.B * a.Hkv + 3) / 4 * 4;
+  const long long dkv = kv > 1 ? (long long)kv * a.B * a.Hkv * a.Tk * a.D : 0;
+  const long long dq = q > 1 ? (long long)q * a.B * a.Hq * a.Tq * a.D : 0;
+  if (p) {
+    float* w = static_cast<float*>(a.workspace);
+    p->delta = w;
+    p->lse2 = w + rows;
+    p->norm_bits = reinterpret_cast<unsigned*>(w + 2 * rows);
+    p->part_dk = w + 2 * rows + bits;
+    p->part_dv = p->part_dk + dkv;
+    p->part_dq = p->part_dv + dkv;
+    p->kv_splits = kv;
+    p->q_splits = q;
+  }
+  return (2 * rows + bits + 2 * dkv + dq) * (long long)sizeof(float);
 }
 
 }  // namespace
 
-long long attn_bwd_bytes(const WubuB200Attn& a) {
-  const long long t_pad = (a.Tq + kTile - 1) / kTile * kTile;
-  return 2ll * a.B * a.Hq * t_pad * (long long)sizeof(float) + 2ll * a.B * a.Hkv * (long long)sizeof(unsigned);
-}
+long long attn_bwd_bytes(const WubuB200Attn& a) { return bwd_layout(a, nullptr); }
 
 int attn_backward(const AttnParams& in, cudaStream_t st) {
   AttnParams p = in;
   const WubuB200Attn& a = p.a;
-  const long long rows = (long long)a.B * a.Hq * p.t_pad;
-  p.delta = static_cast<float*>(a.workspace);
-  p.lse2 = p.delta + rows;
-  p.norm_bits = reinterpret_cast<unsigned*>(p.lse2 + rows);
+  bwd_layout(a, &p);
+  const int sms = attn_sms();
+  if (!sms) return WUBU_B200_ERR_CUDA;
   AttnBwdMaps maps{};
   if (a.Tq && (!attn_map(&maps.q, a.q, a.B, a.Tq, a.Hq, a.D) || !attn_map(&maps.dout, a.dout, a.B, a.Tq, a.Hq, a.D)))
     return WUBU_B200_ERR_CUDA;
   if (a.Tk && (!attn_map(&maps.k, a.k, a.B, a.Tk, a.Hkv, a.D) || !attn_map(&maps.v, a.v, a.B, a.Tk, a.Hkv, a.D)))
     return WUBU_B200_ERR_CUDA;
   if (a.dtype == WUBU_B200_BF16)
-    return a.D <= 64 ? launch_bwd<bf16, 64>(maps, p, st) : launch_bwd<bf16, 128>(maps, p, st);
-  return a.D <= 64 ? launch_bwd<f16, 64>(maps, p, st) : launch_bwd<f16, 128>(maps, p, st);
+    return a.D <= 64 ? launch_bwd<bf16, 64>(maps, p, sms, st) : launch_bwd<bf16, 128>(maps, p, sms, st);
+  return a.D <= 64 ? launch_bwd<f16, 64>(maps, p, sms, st) : launch_bwd<f16, 128>(maps, p, sms, st);
 }
 
 }  // namespace wb

@@ -29,6 +29,28 @@ inline int ops_launched(const char* what) {
   return WUBU_B200_ERR_CUDA;
 }
 
+// Launches a kernel that may start while its predecessor on the stream still runs (it waits for it with
+// griddep_wait before it touches what that wrote).
+template <typename... Args, typename... Given>
+int ops_launch_after(void (*kernel)(Args...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const char* what,
+                     Given... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, Args(args)...);
+  if (e == cudaSuccess) return WUBU_B200_OK;
+  cudaGetLastError();
+  fprintf(stderr, "wuburvc_b200: %s launch failed: %s\n", what, cudaGetErrorString(e));
+  return WUBU_B200_ERR_CUDA;
+}
+
 inline bool ops_dtype_ok(int dtype) {
   return dtype == WUBU_B200_F32 || dtype == WUBU_B200_BF16 || dtype == WUBU_B200_F16;
 }
