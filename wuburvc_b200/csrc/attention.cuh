@@ -7,8 +7,9 @@ namespace wb {
 struct AttnParams {
   WubuB200Attn a;    // with scale resolved and strides of unit extents cleared
   int group;         // query heads to a key / value head
-  float* delta;      // backward: [B][Hq][t_pad] rowsum(dO * O)
-  float* lse2;       // backward: [B][Hq][t_pad] lse in units of log 2; +infinity where a query sees nothing
+  float* delta;      // backward: [B][Hq][t_pad] - rowsum(dO * O)
+  float* lse2;       //           the negative log-sum-exp in units of log 2; -infinity where a query sees nothing
+  unsigned* counter;    // backward: items drawn
   unsigned* norm_bits;  // backward, fp16: [2][B][Hkv] bits of the largest squared row norms of dO and of V
   int t_pad;
   int splits;        // forward: parts that the keys are split into, each with an out and an lse of its own
@@ -113,21 +114,22 @@ WB_DEV void mma4_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// The same with A in tensor memory (128 rows, two 16-bit values a column) and B along its tokens (16 tokens
-// are 2 KB).
+// The same with A in tensor memory (128 rows, two 16-bit values a column, the second pair of steps at column A2)
+// and B along its tokens (16 tokens are 2 KB).
+template <int A2 = 16>
 WB_DEV void mma4_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p, e;\n\t.reg .b64 b1, b2, b3;\n\t.reg .b32 a1, a2, a3;\n\t"
       "elect.sync _|e, 0xffffffff;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "add.u32 a1, %1, 8;\n\tadd.u64 b1, %2, 128;\n\t"
-      "add.u32 a2, %1, 16;\n\tadd.u64 b2, %2, 256;\n\t"
-      "add.u32 a3, %1, 24;\n\tadd.u64 b3, %2, 384;\n\t"
+      "add.u32 a2, %1, %5;\n\tadd.u64 b2, %2, 256;\n\t"
+      "add.u32 a3, a2, 8;\n\tadd.u64 b3, %2, 384;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, 1;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, 1;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, 1;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "n"(A2)
       : "memory");
 }
 // D[tmem] = A B^T over the values of two tiles; `ksteps` (at most DP / 16) steps of 16
@@ -207,6 +209,11 @@ WB_DEV void tmem_st16(uint32_t taddr, const uint32_t* r) {
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
       : "memory");
 }
+WB_DEV void tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+               : "memory");
+}
 WB_DEV void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -223,23 +230,26 @@ WB_DEV bool bar_wait(uint64_t* bar, uint32_t parity, int* err, int code, unsigne
   if (__all_sync(0xffffffffu, done)) return true;
   return mbar_wait_warp(bar, parity, err, code, limit_ns);
 }
-// A warp writes 32 rows x 32 values, a row in each lane (packed pairs w[16]), 64 bytes to a row at a time: through
-// 2 KB of shared memory, 16-byte pieces swizzled by row, then four lanes to a row.  `row` is the first
-// row's address, rows are `stride` elements apart; rows from `rows` and values from `cols` on are left out.
-// (Each lane storing its own row touched 32 lines an instruction and took several thousand cycles a tile.)
-template <typename T>
+// A warp writes 32 rows x 8 N values, a row in each lane (packed pairs w[4 N]), 16 N bytes to a row at a time:
+// through 512 N bytes of shared memory, 16-byte pieces swizzled by row, then N lanes to a row.  `row` is the
+// first row's address, rows are `stride` elements apart; rows from `rows` and values from `cols` on are
+// left out.  (Each lane storing its own row touched 32 lines an instruction and took several thousand
+// cycles a tile.)
+template <int N, typename T>
 WB_DEV void store_rows(uint8_t* stage, const uint32_t* w, T* row, long long stride, int rows, int cols) {
+  static_assert(N == 2 || N == 4, "");
+  constexpr int kSkew = N == 4 ? 1 : 2;  // rows apart by 128 bytes take other pieces
   const int lane = threadIdx.x & 31;
   uint4* st = reinterpret_cast<uint4*>(stage);
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
-    st[lane * 4 + (c ^ (lane >> 1 & 3))] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+  for (int c = 0; c < N; ++c)
+    st[lane * N + (c ^ (lane >> kSkew & (N - 1)))] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
   __syncwarp();
-  const int c = lane & 3;
+  const int c = lane & (N - 1);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 8 * i + (lane >> 2);
-    const uint4 v = st[r * 4 + (c ^ (r >> 1 & 3))];
+  for (int i = 0; i < N; ++i) {
+    const int r = 32 / N * i + lane / N;
+    const uint4 v = st[r * N + (c ^ (r >> kSkew & (N - 1)))];
     if (r < rows && c * 8 < cols) *reinterpret_cast<uint4*>(row + r * stride + c * 8) = v;
   }
   __syncwarp();

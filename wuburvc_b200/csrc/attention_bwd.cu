@@ -11,7 +11,7 @@
 //
 // Everything between the products stays in tensor memory.  The first role forms the transposed scores
 // (rows are keys), so that P^T and dS^T are written over them as the A operands of the next products.
-// Eight warps do the exponentials, two to a row quadrant, 64 columns a thread; one warp loads, one
+// Sixteen warps do the exponentials, four to a row quadrant, 32 columns a thread; one warp loads, one
 // issues.  A CTA an SM works through the items of both roles, loading the next one's tiles behind the last
 // one's steps; where one item would outlast the rest, its steps are split and float32 parts joined.  A step's products and its elementwise halves alternate:
 //   keys' role:     tensor  dV(n) S(n+1) | dK(n) dP(n+1)      warps  dS(n) | P(n+1)
@@ -26,7 +26,7 @@
 namespace wb {
 namespace {
 
-constexpr int kProducer = 8, kMma = 9, kThreads = 384;
+constexpr int kProducer = 16, kMma = 17, kThreads = 640;  // 640 x 96 registers = 512 x 104 + 128 x 64
 constexpr float kLog2e = 1.4426950408889634f;
 // Tiles in the ring of Q or K, and of dO or V.  (Of K the second role wants a third, which 128 values a row
 // leave no room for beside the store staging.)
@@ -48,7 +48,7 @@ struct BwdShift<f16> {
 };
 
 struct Barriers {
-  uint64_t res_full, res_empty, a_full[3], a_empty[3], b_full[kStagesB], b_empty[kStagesB], s_full[2], dp_full, p_ready,
+  uint64_t item_full[2], item_empty[2], res_full, res_empty, a_full[3], a_empty[3], b_full[kStagesB], b_empty[kStagesB], s_full[2], dp_full, p_ready,
       ds_ready, acc_full, acc_read, mma_done;
 };
 
@@ -115,7 +115,35 @@ WB_DEV float ds_scale(const AttnParams& p, int b, int hk) {
   return exp2f(fminf(floorf(log2f(16384.f / m)), 100.f));
 }
 
+WB_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
 // SPLIT: in one role at least the steps of an item are split.
+// The CTAs take items in order as they come free (the lengths and causal order make items unequal): the first by
+// their number, the rest from a counter that the kernel before has cleared.  The loading warp draws and
+// hands the number to the other warps.  Which CTA works on an item does not change its result.
+struct Items {
+  Barriers& bar;
+  volatile int* slots;
+  int n;  // taken so far
+  WB_DEV bool take(int& id, const AttnParams& p, int work) {
+    const int s = n & 1;
+    const bool ok = bar_wait(&bar.item_full[s], (n >> 1) & 1, p.err, ERR_WAIT_FULL, p.wait_ns);
+    id = ok ? slots[s] : work;
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&bar.item_empty[s]);
+    ++n;
+    return id < work;
+  }
+};
+
 template <typename T, int DP, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_constant__ AttnParams p, int kv_work, int work) {
@@ -130,13 +158,20 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
   uint8_t* res1 = smem + kTileBytes;       // V or dO
   uint8_t* ra = smem + 2 * kTileBytes;     // ring of Q or K
   uint8_t* rb = ra + kA * kTileBytes;      // ring of dO or V
-  uint8_t* stage = rb + kStagesB * kTileBytes;  // 2 KB a warp
+  uint8_t* stage = rb + kStagesB * kTileBytes;  // 1 KB a warp
+  // keys' role: the log-sum-exp and row sum of a step's 128 queries, with the first ring's tiles
+  float* rows = reinterpret_cast<float*>(stage + kProducer * 1024);
   __shared__ Barriers bar;
+  __shared__ int item_slots[2];
   __shared__ uint32_t tmem_slot;
 
   const WubuB200Attn& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.item_full[i], 1);
+      mbar_init(&bar.item_empty[i], kProducer + 1);
+    }
     mbar_init(&bar.res_full, 1);
     mbar_init(&bar.res_empty, 1);
     for (int i = 0; i < kA; ++i) {
@@ -150,10 +185,10 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
     mbar_init(&bar.s_full[0], 1);
     mbar_init(&bar.s_full[1], 1);
     mbar_init(&bar.dp_full, 1);
-    mbar_init(&bar.p_ready, 8);
-    mbar_init(&bar.ds_ready, 8);
+    mbar_init(&bar.p_ready, kProducer);
+    mbar_init(&bar.ds_ready, kProducer);
     mbar_init(&bar.acc_full, 1);
-    mbar_init(&bar.acc_read, 8);
+    mbar_init(&bar.acc_read, kProducer);
     mbar_init(&bar.mma_done, 1);
     fence_barrier_init();
   }
@@ -165,13 +200,26 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
   const uint32_t tDP = tmem + 128, tAcc0 = tmem + 256, tAcc1 = tmem + 384;
 
   if (warp >= kProducer) {
-    regs_dec<72>();
+    regs_dec<64>();
     if (warp == kProducer) {
       bool ok = true;
       FillTrack fr, fa, fb;
-      int n = 0, items = 0;  // steps and items (with steps) so far
-      for (AttnRounds r(work); r.more(); r.advance()) {
-        const BwdWork k(p, r.next, kv_work);
+      int n = 0, items = 0, drawn = 0;  // steps, items with steps, and all items so far
+      int next = blockIdx.x;
+      for (;;) {
+        int id = __shfl_sync(0xffffffffu, next, 0);
+        if (ok && drawn >= 2) ok = bar_wait(&bar.item_empty[drawn & 1], ((drawn >> 1) & 1) ^ 1u, p.err, ERR_WAIT_EMPTY, p.wait_ns);
+        if (!ok) id = work;
+        if (lane == 0) {
+          item_slots[drawn & 1] = id;
+          mbar_arrive(&bar.item_full[drawn & 1]);
+        }
+        __syncwarp();
+        if (id >= work) break;
+        const BwdWork k(p, id, kv_work);
+        if (drawn++ == 0) griddep_wait();  // the counter, the row sums and log-sum-exps come from the kernel before
+        // (drawn here, looked at when the item's loads are out)
+        next = lane == 0 ? (int)gridDim.x + (int)atomicAdd(p.counter, 1u) : 0;
         if (k.steps == 0) continue;
         if (ok && items) ok = bar_wait(&bar.res_empty, (items - 1) & 1, p.err, ERR_WAIT_EMPTY, p.wait_ns);
         if (ok) {
@@ -188,8 +236,13 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
           if (ok && n >= kA) ok = bar_wait(&bar.a_empty[sa], pa ^ 1u, p.err, ERR_WAIT_EMPTY, p.wait_ns);
           if (ok) {
             fa.fill(sa, pa);
-            mbar_expect_tx_warp(&bar.a_full[sa], kTileBytes);
+            mbar_expect_tx_warp(&bar.a_full[sa], kTileBytes + (k.kv ? 2 * kTile * 4 : 0));
             load_tile(ra + sa * kTileBytes, k.kv ? &maps.q : &maps.k, &bar.a_full[sa], t * kTile, h, k.b, kBoxes);
+            if (k.kv) {
+              const long long q = ((long long)k.b * a.Hq + h) * p.t_pad + t * kTile;
+              bulk_load(rows + sa * 2 * kTile, p.lse2 + q, kTile * 4, &bar.a_full[sa]);
+              bulk_load(rows + sa * 2 * kTile + kTile, p.delta + q, kTile * 4, &bar.a_full[sa]);
+            }
           }
           if (ok && n >= kStagesB) ok = bar_wait(&bar.b_empty[sb], pb ^ 1u, p.err, ERR_WAIT_EMPTY, p.wait_ns);
           if (ok) {
@@ -211,8 +264,9 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
       bool ok = true;
       int n0 = 0, items = 0, p_count = 0;
       int all = 0;  // items so far, those without steps too
-      for (AttnRounds r(work); r.more(); r.advance(), ++all) {
-        const BwdWork k(p, r.next, kv_work);
+      Items take{bar, item_slots, 0};
+      for (int id; take.take(id, p, work); ++all) {
+        const BwdWork k(p, id, kv_work);
         if (k.steps == 0) continue;
         const bool kv = k.kv;
         if (ok) ok = bar_wait(&bar.res_full, items & 1, p.err, ERR_WAIT_FULL, p.wait_ns);
@@ -245,11 +299,11 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
             if (i == k.steps - 1) umma_commit_warp(&bar.res_empty);
           }
         };
-        // acc += (A in tensor memory, 128 x 128, its halves 64 columns apart) x tile
+        // acc += (A in tensor memory, 128 x 128, its quarters 32 columns apart) x tile
         auto issue_acc = [&](uint32_t acc, uint32_t src, const uint8_t* tile, int i) {
           const uint64_t d = desc_mn(tile);
-          mma4_ts(acc, src, d, id_o, i > 0);
-          mma4_ts(acc, src + 64, d + (4 * 2048u >> 4), id_o, 1);
+          mma4_ts<32>(acc, src, d, id_o, i > 0);
+          mma4_ts<32>(acc, src + 64, d + (4 * 2048u >> 4), id_o, 1);
         };
         issue_s(0);
         issue_dp(0);
@@ -286,149 +340,165 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
       bar_wait(&bar.mma_done, 0, p.err, ERR_WAIT_ACC, p.wait_ns);
     }
   } else {
-    regs_inc<216>();
-    const int half = warp >> 2;
+    regs_inc<104>();
+    const int quarter = warp >> 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t DPc = tDP + lanes + 64 * half;
+    const uint32_t DPc = tDP + lanes + 32 * quarter;
     const float c = a.scale * kLog2e;
     bool ok = true;
     int n0 = 0, items = 0;         // steps and items (with steps) so far
     uint32_t s_phase[2] = {0, 0};  // of the two buffers of S
-    griddep_wait();                // the row sums and log-sum-exps come from the kernel before
-    for (AttnRounds r(work); r.more(); r.advance()) {
-      const BwdWork k(p, r.next, kv_work);
-      const bool kv = k.kv;
-      const AttnItem it = k.it;
-      const int row = k.own0 + (warp & 3) * 32 + lane;  // a key or a query
-      const int lo = kv ? it.query_lo(a, row) : it.key_lo(a, row), hi = kv ? it.query_hi(a, row) : it.key_hi(a, row);
-      // tiles that all of this tile's live rows meet whole need no mask
-      const int last = min(k.own0 + kTile, kv ? it.kl : it.ql) - 1;
-      const int all_lo = last >= k.own0 ? (kv ? it.query_lo(a, last) : it.key_lo(a, last)) : 0;
-      const int all_hi = kv ? it.query_hi(a, k.own0) : it.key_hi(a, k.own0);
-      const float f = kBf16 ? 1.f : ds_scale<T>(p, k.b, k.hk) * exp2f(-kShift);  // on P 2^shift (dP - D)
-      float l2 = 0.f, delta = 0.f;
-      if (!kv && k.steps > 0) {
-        const long long q = ((long long)k.b * a.Hq + k.hq) * p.t_pad + row;
-        l2 = p.lse2[q];
-        delta = p.delta[q];
-      }
-      int t = k.t, h = k.h;
-      for (int i = 0; i < k.steps; ++i) {
-        const int col0 = t * kTile + 64 * half, buf = kv ? 0 : i & 1;
-        const uint32_t S = tmem + 256 * buf + lanes + 64 * half;
-        const long long q0 = ((long long)k.b * a.Hq + h) * p.t_pad + col0;  // keys' role: the step's queries
-        const bool masked = t * kTile < all_lo || t * kTile + kTile > all_hi;
-        k.advance(t, h);
-        float rows[64];
-        if (kv) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) *reinterpret_cast<float4*>(rows + 4 * e) = *reinterpret_cast<const float4*>(p.lse2 + q0 + 4 * e);
+    griddep_wait();                // the queries' role reads row sums and log-sum-exps itself
+    Items take{bar, item_slots, 0};
+    for (int id; take.take(id, p, work);) {
+      bool kv;
+      int steps, t, t0, t_end;             // steps; the next step's tile, and the range that it runs through
+      int lo, hi, whole0, whole1;          // the row's range, and the tiles that need no mask
+      float l2 = 0.f, delta = 0.f, f = 1.f;  // queries' role: the row's values; the scale of P 2^shift (dP - D)
+      {
+        const BwdWork k(p, id, kv_work);
+        kv = k.kv;
+        steps = k.steps;
+        t = k.t;
+        t0 = k.t0;
+        t_end = k.t0 + k.per_head;
+        const int row = k.own0 + (warp & 3) * 32 + lane;  // a key or a query
+        lo = kv ? k.it.query_lo(a, row) : k.it.key_lo(a, row);
+        hi = kv ? k.it.query_hi(a, row) : k.it.key_hi(a, row);
+        // tiles that all of this tile's live rows meet whole
+        const int last = min(k.own0 + kTile, kv ? k.it.kl : k.it.ql) - 1;
+        const int all_lo = last >= k.own0 ? (kv ? k.it.query_lo(a, last) : k.it.key_lo(a, last)) : 0;
+        const int all_hi = kv ? k.it.query_hi(a, k.own0) : k.it.key_hi(a, k.own0);
+        whole0 = (all_lo + kTile - 1) / kTile;
+        whole1 = all_hi / kTile;
+        if (!kBf16) f = ds_scale<T>(p, k.b, k.hk) * exp2f(-kShift);
+        if (!kv && steps > 0) {
+          const long long q = ((long long)k.b * a.Hq + k.hq) * p.t_pad + row;
+          l2 = p.lse2[q];
+          delta = p.delta[q];
         }
+      }
+      for (int i = 0; i < steps; ++i) {
+        const int col0 = t * kTile + 32 * quarter, n = n0 + i, buf = kv ? 0 : i & 1;
+        const bool masked = t < whole0 || t >= whole1;
+        if (++t == t_end) t = t0;
+        const uint32_t S = tmem + 256 * buf + lanes + 32 * quarter;
+        const float4* step_rows = reinterpret_cast<const float4*>(rows + n % kA * 2 * kTile + 32 * quarter);
+        if (kv && ok) ok = bar_wait(&bar.a_full[n % kA], (n / kA) & 1, p.err, ERR_WAIT_FULL, p.wait_ns);
         if (ok) ok = bar_wait(&bar.s_full[buf], buf ? s_phase[1] : s_phase[0], p.err, ERR_WAIT_ACC, p.wait_ns);
         if (buf) s_phase[1] ^= 1u;
         else s_phase[0] ^= 1u;
         if (!ok) continue;
         tc_fence_after();
-        float x[64];
-        tmem_load<64>(S, x);
+        float x[32];
+        tmem_load<32>(S, x);
+        const uint64_t cc = two(c, c);
         if (kv) {
 #pragma unroll
-          for (int e = 0; e < 64; ++e) x[e] = ex2(fmaf(x[e], c, kShift - rows[e]));
+          for (int e = 0; e < 8; ++e) {
+            const float4 v = step_rows[e];
+            each(fma2(two(x[4 * e], x[4 * e + 1]), cc, two(v.x, v.y)), x[4 * e], x[4 * e + 1]);
+            each(fma2(two(x[4 * e + 2], x[4 * e + 3]), cc, two(v.z, v.w)), x[4 * e + 2], x[4 * e + 3]);
+          }
         } else {
-          const uint64_t cc = two(c, c), ll = two(kShift - l2, kShift - l2);
 #pragma unroll
-          for (int e = 0; e < 64; e += 2) each(fma2(two(x[e], x[e + 1]), cc, ll), x[e], x[e + 1]);
-#pragma unroll
-          for (int e = 0; e < 64; ++e) x[e] = ex2(x[e]);
+          for (int e = 0; e < 32; e += 2) each(fma2(two(x[e], x[e + 1]), cc, two(l2, l2)), x[e], x[e + 1]);
         }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = ex2(x[e]);
         if (masked) {
+          const uint32_t see = see_bits(lo - col0, hi - col0);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = see >> e & 1 ? x[e] : 0.f;
+        }
+        if (kv) {
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
-            const uint32_t see = see_bits(lo - col0 - 32 * g, hi - col0 - 32 * g);
+            uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) x[32 * g + e] = see >> e & 1 ? x[32 * g + e] : 0.f;
+            for (int e = 0; e < 8; ++e) w[e] = pack2(x[16 * g + 2 * e], x[16 * g + 2 * e + 1], T());
+            tmem_st8(S + 8 * g, w);
           }
-        }
-        if (kv) {
-          uint32_t w[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) w[e] = pack2(x[2 * e], x[2 * e + 1], T());
-          tmem_st32(S, w);
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar.p_ready);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) *reinterpret_cast<float4*>(rows + 4 * e) = *reinterpret_cast<const float4*>(p.delta + q0 + 4 * e);
         }
-        ok = bar_wait(&bar.dp_full, (n0 + i) & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
+        ok = bar_wait(&bar.dp_full, n & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
         if (!ok) continue;
         tc_fence_after();
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          float y[32];
-          uint32_t w[16];
-          tmem_load<32>(DPc + 32 * g, y);
+        for (int g = 0; g < 2; ++g) {  // 16 columns at a time, written over columns that have been read
+          float y[16];
+          uint32_t w[8];
+          tmem_load16(DPc + 16 * g, y);
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float* d = rows + 32 * g + e;
-            uint64_t v = add2(two(y[e], y[e + 1]), kv ? two(-d[0], -d[1]) : two(-delta, -delta));
-            v = mul2(v, two(x[32 * g + e], x[32 * g + e + 1]));
-            if (!kBf16) v = mul2(v, two(f, f));
-            each(v, y[e], y[e + 1]);
-            w[e / 2] = pack2(y[e], y[e + 1], T());
+          for (int e = 0; e < 4; ++e) {
+            const float* xe = x + 16 * g + 4 * e;
+            const float4 v = kv ? step_rows[kTile / 4 + 4 * g + e] : make_float4(delta, delta, delta, delta);
+            uint64_t g0 = mul2(add2(two(y[4 * e], y[4 * e + 1]), two(v.x, v.y)), two(xe[0], xe[1]));
+            uint64_t g1 = mul2(add2(two(y[4 * e + 2], y[4 * e + 3]), two(v.z, v.w)), two(xe[2], xe[3]));
+            if (!kBf16) {
+              g0 = mul2(g0, two(f, f));
+              g1 = mul2(g1, two(f, f));
+            }
+            float u0, u1, u2, u3;
+            each(g0, u0, u1);
+            each(g1, u2, u3);
+            w[2 * e] = pack2(u0, u1, T());
+            w[2 * e + 1] = pack2(u2, u3, T());
           }
-          tmem_st16(DPc + 16 * g, w);  // over columns that have been read
+          tmem_st8(DPc + 8 * g, w);
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.ds_ready);
       }
+      asm volatile("" : "+r"(id));  // (formed again rather than held in registers over the steps)
+      const BwdWork k(p, id, kv_work);
       n0 += k.steps;
       if (k.steps > 0) {
         if (ok) ok = bar_wait(&bar.acc_full, items & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
         ++items;
         tc_fence_after();
       }
-      // the accumulators, half of the columns to each warpgroup
+      // the accumulators, a quarter of the columns to each warpgroup
+      const int row = k.own0 + (warp & 3) * 32 + lane;
       const bool live = hi > lo && k.steps > 0 && ok;
       const float ds_out = a.scale / (kBf16 ? 1.f : f * exp2f(kShift)), p_out = exp2f(-kShift);
-      const int d0 = DP / 2 * half;
+      constexpr int kCols = DP / 4;
+      const int d0 = kCols * quarter;
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
         if (!kv && which == 0) continue;
         const float sc = which ? ds_out : p_out;
-        auto values = [&](int d, float* o) {  // 32 of the row's results, from d0 + d
-          if (k.steps > 0) tmem_load<32>((which ? tAcc1 : tAcc0) + lanes + d0 + d, o);
+        float o[kCols];
+        if (k.steps > 0) {
+          const uint32_t at_ = (which ? tAcc1 : tAcc0) + lanes + d0;
+          if (kCols == 32) tmem_load<32>(at_, o);
+          else tmem_load16(at_, o);
+        }
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = live ? o[e] * sc : 0.f;
-        };
+        for (int e = 0; e < kCols; ++e) o[e] = live ? o[e] * sc : 0.f;
+        const int tokens = kv ? a.Tk : a.Tq, H = kv ? a.Hkv : a.Hq, head = kv ? k.hk : k.hq;
         if (SPLIT && (kv ? p.kv_splits : p.q_splits) > 1) {
-          const long long T_ = kv ? a.Tk : a.Tq, H = kv ? a.Hkv : a.Hq, all = a.B * H * T_ * a.D;
-          float* part = (!kv ? p.part_dq : which ? p.part_dk : p.part_dv) + k.split * all +
-                        (((long long)k.b * H + (kv ? k.hk : k.hq)) * T_ + row) * a.D + d0;
+          float* part = (!kv ? p.part_dq : which ? p.part_dk : p.part_dv) +
+                        ((((long long)k.split * a.B + k.b) * H + head) * tokens + row) * a.D + d0;
 #pragma unroll
-          for (int d = 0; d < DP / 2; d += 32) {
-            float o[32];
-            values(d, o);
-#pragma unroll
-            for (int e = 0; e < 32; e += 8)
-              if (row < T_ && d0 + d + e < a.D) store8(part + d + e, o + e);
-            __syncwarp();
-          }
+          for (int e = 0; e < kCols; e += 8)
+            if (row < tokens && d0 + e < a.D) store8(part + e, o + e);
+          __syncwarp();
         } else {
           const int r0 = k.own0 + (warp & 3) * 32;
           const WubuB200View& view = !kv ? a.dq : which ? a.dk : a.dv;
-          T* out = at<T>(view, k.b, r0, kv ? k.hk : k.hq) + d0;
+          T* out = at<T>(view, k.b, r0, head) + d0;
 #pragma unroll
-          for (int d = 0; d < DP / 2; d += 32) {
-            float o[32];
-            values(d, o);
-            uint32_t w[16];
+          for (int g = 0; g < kCols; g += 16) {
+            uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) w[e] = pack2(o[2 * e], o[2 * e + 1], T());
-            store_rows(stage + warp * 2048, w, out + d, view.token, (kv ? a.Tk : a.Tq) - r0, a.D - d0 - d);
+            for (int e = 0; e < 8; ++e) w[e] = pack2(o[g + 2 * e], o[g + 2 * e + 1], T());
+            store_rows<2>(stage + warp * 1024, w, out + g, view.token, tokens - r0, a.D - d0 - g);
           }
         }
       }
@@ -452,13 +522,14 @@ WB_DEV float dot8(const T* x, const T* y) {
   return s;
 }
 
-// delta = rowsum(dO * O) and the log-sum-exp in units of log 2, padded to whole tiles with what gives
-// probability 0; for fp16 also the largest squared norms of dO's and V's rows (an integer maximum over
+// - rowsum(dO * O) and the negative log-sum-exp in units of log 2 (with P's shift), padded to whole tiles with
+// what gives probability 0; for fp16 also the largest squared norms of dO's and V's rows (an integer maximum over
 // the bits of non-negative floats: its order does not matter).  N threads a row, 8 values each.
 template <typename T, int N>
 __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnParams p) {
   const WubuB200Attn& a = p.a;
   const int t = threadIdx.x % N, i = blockIdx.x * (256 / N) + threadIdx.x / N, h = blockIdx.y, b = blockIdx.z;
+  if (threadIdx.x == 0 && blockIdx.x == 0 && h == 0 && b == 0) *p.counter = 0;
   const AttnItem it(a, b);
   constexpr bool kNorms = std::is_same<T, f16>::value;
   float d = 0.f, g = 0.f, v = 0.f;
@@ -482,8 +553,8 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnParams p) {
   if (t == 0 && i < p.t_pad) {
     const long long r = ((long long)b * a.Hq + h) * p.t_pad + i;
     const float l = i < it.ql ? a.lse[((long long)b * a.Hq + h) * a.Tq + i] * kLog2e : INFINITY;
-    p.delta[r] = d;
-    p.lse2[r] = l == -INFINITY ? INFINITY : l;
+    p.delta[r] = -d;
+    p.lse2[r] = l == -INFINITY ? -INFINITY : BwdShift<T>::value - l;
   }
   if (kNorms) {
     const int n = a.B * a.Hkv, at_ = b * a.Hkv + h / p.group;
@@ -538,7 +609,7 @@ void bwd_splits(const WubuB200Attn& a, int sms, int& kv, int& q) {
 template <typename T, int DP>
 int launch_bwd(const AttnBwdMaps& maps, const AttnParams& p, int sms, cudaStream_t st) {
   const WubuB200Attn& a = p.a;
-  constexpr int smem = (2 + kStagesA<DP> + kStagesB) * (DP / 64) * (int)kBox + 8 * 2048 + 1024;
+  constexpr int smem = (2 + kStagesA<DP> + kStagesB) * (DP / 64) * (int)kBox + kProducer * 1024 + kStagesA<DP> * 2 * kTile * 4 + 1024;
   static std::atomic<uint64_t> devices[2];
   auto* kernel = p.kv_splits > 1 || p.q_splits > 1 ? attn_bwd_tc_kernel<T, DP, true> : attn_bwd_tc_kernel<T, DP, false>;
   if (!ops_smem_limit((const void*)attn_bwd_tc_kernel<T, DP, true>, smem, devices[0]) ||
@@ -549,7 +620,7 @@ int launch_bwd(const AttnBwdMaps& maps, const AttnParams& p, int sms, cudaStream
     return WUBU_B200_ERR_CUDA;
   const int rows = std::is_same<T, f16>::value && a.Tk > p.t_pad ? a.Tk : p.t_pad;
   constexpr int kRows = 256 / (DP / 8);
-  if (rows) attn_delta_kernel<T, DP / 8><<<dim3((rows + kRows - 1) / kRows, a.Hq, a.B), 256, 0, st>>>(p);
+  attn_delta_kernel<T, DP / 8><<<dim3(rows ? (rows + kRows - 1) / kRows : 1, a.Hq, a.B), 256, 0, st>>>(p);
   int rc = ops_launched("attn_backward rows");
   if (rc != WUBU_B200_OK) return rc;
   const long long kv = tiles_of(a.Tk) * a.Hkv * a.B * p.kv_splits, qs = tiles_of(a.Tq) * a.Hq * a.B * p.q_splits;
@@ -569,18 +640,19 @@ int launch_bwd(const AttnBwdMaps& maps, const AttnParams& p, int sms, cudaStream
   return rc;
 }
 
-// The workspace: delta, lse2, norm bits (to a multiple of 16 bytes), then the parts of dk, dv and dq.
+// The workspace: delta, lse2, counter and norm bits (to a multiple of 16 bytes), then the parts of dk, dv and dq.
 long long bwd_layout(const WubuB200Attn& a, AttnParams* p) {
   int kv = 1, q = 1;
   bwd_splits(a, attn_sms(), kv, q);
-  const long long rows = (long long)a.B * a.Hq * tiles_of(a.Tq) * kTile, bits = (2ll * a.B * a.Hkv + 3) / 4 * 4;
+  const long long rows = (long long)a.B * a.Hq * tiles_of(a.Tq) * kTile, bits = (1 + 2ll * a.B * a.Hkv + 3) / 4 * 4;
   const long long dkv = kv > 1 ? (long long)kv * a.B * a.Hkv * a.Tk * a.D : 0;
   const long long dq = q > 1 ? (long long)q * a.B * a.Hq * a.Tq * a.D : 0;
   if (p) {
     float* w = static_cast<float*>(a.workspace);
     p->delta = w;
     p->lse2 = w + rows;
-    p->norm_bits = reinterpret_cast<unsigned*>(w + 2 * rows);
+    p->counter = reinterpret_cast<unsigned*>(w + 2 * rows);
+    p->norm_bits = p->counter + 1;
     p->part_dk = w + 2 * rows + bits;
     p->part_dv = p->part_dk + dkv;
     p->part_dq = p->part_dv + dkv;

@@ -405,7 +405,7 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
           uint32_t w[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) w[k] = pack2(o[2 * k], o[2 * k + 1], T());
-          store_rows(stage + warp * 2048, w, out + d0, a.out.token, a.Tq - r0, a.D - d0);
+          store_rows<4>(stage + warp * 2048, w, out + d0, a.out.token, a.Tq - r0, a.D - d0);
         }
       }
       tc_fence_before();  // O is read before the next item's first product may be issued
