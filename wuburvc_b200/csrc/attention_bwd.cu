@@ -319,7 +319,10 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
             if (ok) ok = bar_wait(&bar.p_ready, p_count & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
             ++p_count;
             tc_fence_after();
-            if (ok) issue_acc(tAcc0, tmem, rb + sb * kTileBytes, i);
+            if (ok) {
+              issue_acc(tAcc0, tmem, rb + sb * kTileBytes, i);
+              umma_commit_warp(&bar.b_empty[sb]);
+            }
             if (i + 1 < k.steps) issue_s(i + 1);
           }
           if (ok) ok = bar_wait(&bar.ds_ready, n & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
@@ -327,7 +330,6 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
           if (ok) {
             issue_acc(tAcc1, tDP, ra + sa * kTileBytes, i);
             umma_commit_warp(&bar.a_empty[sa]);
-            if (kv) umma_commit_warp(&bar.b_empty[sb]);
             if (i == k.steps - 1) umma_commit_warp(&bar.acc_full);
           }
           if (i + 1 < k.steps) issue_dp(i + 1);
@@ -378,83 +380,104 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
           delta = p.delta[q];
         }
       }
-      for (int i = 0; i < steps; ++i) {
-        const int col0 = t * kTile + 32 * quarter, n = n0 + i, buf = kv ? 0 : i & 1;
-        const bool masked = t < whole0 || t >= whole1;
-        if (++t == t_end) t = t0;
-        const uint32_t S = tmem + 256 * buf + lanes + 32 * quarter;
-        const float4* step_rows = reinterpret_cast<const float4*>(rows + n % kA * 2 * kTile + 32 * quarter);
-        if (kv && ok) ok = bar_wait(&bar.a_full[n % kA], (n / kA) & 1, p.err, ERR_WAIT_FULL, p.wait_ns);
-        if (ok) ok = bar_wait(&bar.s_full[buf], buf ? s_phase[1] : s_phase[0], p.err, ERR_WAIT_ACC, p.wait_ns);
-        if (buf) s_phase[1] ^= 1u;
-        else s_phase[0] ^= 1u;
-        if (!ok) continue;
-        tc_fence_after();
-        float x[32];
-        tmem_load<32>(S, x);
-        const uint64_t cc = two(c, c);
-        if (kv) {
+      // the steps of one role (compiled for each: choices inside would cost an instruction a value)
+      auto run = [&](auto role) {
+        constexpr bool KV = decltype(role)::value;
+        int sa = n0 % kA;
+        uint32_t pa = (n0 / kA) & 1;
+        for (int i = 0; i < steps; ++i) {
+          const int buf = KV ? 0 : i & 1;
+          const bool masked = t < whole0 || t >= whole1;
+          const int col0 = t * kTile + 32 * quarter;
+          if (++t == t_end) t = t0;
+          const uint32_t S = tmem + 256 * buf + lanes + 32 * quarter;
+          const float4* step_rows = reinterpret_cast<const float4*>(rows + sa * 2 * kTile + 32 * quarter);
+          if (KV) {
+            if (ok) ok = bar_wait(&bar.a_full[sa], pa, p.err, ERR_WAIT_FULL, p.wait_ns);
+            if (++sa == kA) {
+              sa = 0;
+              pa ^= 1u;
+            }
+          }
+          if (ok) ok = bar_wait(&bar.s_full[buf], buf ? s_phase[1] : s_phase[0], p.err, ERR_WAIT_ACC, p.wait_ns);
+          if (buf) s_phase[1] ^= 1u;
+          else s_phase[0] ^= 1u;
+          if (!ok) continue;
+          tc_fence_after();
+          float x[32];
+          tmem_load<32>(S, x);
+          const uint64_t cc = two(c, c), ll = two(l2, l2);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float4 v = step_rows[e];
-            each(fma2(two(x[4 * e], x[4 * e + 1]), cc, two(v.x, v.y)), x[4 * e], x[4 * e + 1]);
-            each(fma2(two(x[4 * e + 2], x[4 * e + 3]), cc, two(v.z, v.w)), x[4 * e + 2], x[4 * e + 3]);
+            uint64_t l01 = ll, l23 = ll;
+            if (KV) {
+              const float4 v = step_rows[e];
+              l01 = two(v.x, v.y);
+              l23 = two(v.z, v.w);
+            }
+            each(fma2(two(x[4 * e], x[4 * e + 1]), cc, l01), x[4 * e], x[4 * e + 1]);
+            each(fma2(two(x[4 * e + 2], x[4 * e + 3]), cc, l23), x[4 * e + 2], x[4 * e + 3]);
           }
-        } else {
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) each(fma2(two(x[e], x[e + 1]), cc, two(l2, l2)), x[e], x[e + 1]);
-        }
+          for (int e = 0; e < 32; ++e) x[e] = ex2(x[e]);
+          if (masked) {
+            const uint32_t see = see_bits(lo - col0, hi - col0);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = ex2(x[e]);
-        if (masked) {
-          const uint32_t see = see_bits(lo - col0, hi - col0);
+            for (int e = 0; e < 32; ++e) x[e] = see >> e & 1 ? x[e] : 0.f;
+          }
+          if (KV) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = see >> e & 1 ? x[e] : 0.f;
-        }
-        if (kv) {
+            for (int g = 0; g < 2; ++g) {
+              uint32_t w[8];
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
+              for (int e = 0; e < 8; ++e) w[e] = pack2(x[16 * g + 2 * e], x[16 * g + 2 * e + 1], T());
+              tmem_st8(S + 8 * g, w);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.p_ready);
+          }
+          ok = bar_wait(&bar.dp_full, (n0 + i) & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
+          if (!ok) continue;
+          tc_fence_after();
+          const uint64_t dd = two(delta, delta), ff = two(f, f);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {  // 16 columns at a time, written over columns that have been read
+            float y[16];
             uint32_t w[8];
+            tmem_load16(DPc + 16 * g, y);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = pack2(x[16 * g + 2 * e], x[16 * g + 2 * e + 1], T());
-            tmem_st8(S + 8 * g, w);
+            for (int e = 0; e < 4; ++e) {
+              const float* xe = x + 16 * g + 4 * e;
+              uint64_t d01 = dd, d23 = dd;
+              if (KV) {
+                const float4 v = step_rows[kTile / 4 + 4 * g + e];
+                d01 = two(v.x, v.y);
+                d23 = two(v.z, v.w);
+              }
+              uint64_t g0 = mul2(add2(two(y[4 * e], y[4 * e + 1]), d01), two(xe[0], xe[1]));
+              uint64_t g1 = mul2(add2(two(y[4 * e + 2], y[4 * e + 3]), d23), two(xe[2], xe[3]));
+              if (!kBf16) {
+                g0 = mul2(g0, ff);
+                g1 = mul2(g1, ff);
+              }
+              float u0, u1, u2, u3;
+              each(g0, u0, u1);
+              each(g1, u2, u3);
+              w[2 * e] = pack2(u0, u1, T());
+              w[2 * e + 1] = pack2(u2, u3, T());
+            }
+            tmem_st8(DPc + 8 * g, w);
           }
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bar.p_ready);
+          if (lane == 0) mbar_arrive(&bar.ds_ready);
         }
-        ok = bar_wait(&bar.dp_full, n & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
-        if (!ok) continue;
-        tc_fence_after();
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {  // 16 columns at a time, written over columns that have been read
-          float y[16];
-          uint32_t w[8];
-          tmem_load16(DPc + 16 * g, y);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float* xe = x + 16 * g + 4 * e;
-            const float4 v = kv ? step_rows[kTile / 4 + 4 * g + e] : make_float4(delta, delta, delta, delta);
-            uint64_t g0 = mul2(add2(two(y[4 * e], y[4 * e + 1]), two(v.x, v.y)), two(xe[0], xe[1]));
-            uint64_t g1 = mul2(add2(two(y[4 * e + 2], y[4 * e + 3]), two(v.z, v.w)), two(xe[2], xe[3]));
-            if (!kBf16) {
-              g0 = mul2(g0, two(f, f));
-              g1 = mul2(g1, two(f, f));
-            }
-            float u0, u1, u2, u3;
-            each(g0, u0, u1);
-            each(g1, u2, u3);
-            w[2 * e] = pack2(u0, u1, T());
-            w[2 * e + 1] = pack2(u2, u3, T());
-          }
-          tmem_st8(DPc + 8 * g, w);
-        }
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.ds_ready);
-      }
+      };
+      if (kv) run(std::true_type());
+      else run(std::false_type());
       asm volatile("" : "+r"(id));  // (formed again rather than held in registers over the steps)
       const BwdWork k(p, id, kv_work);
       n0 += k.steps;
