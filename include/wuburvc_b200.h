@@ -343,7 +343,10 @@ int wubu_b200_ops_sync(void* stream);
  *             restored as NaN.
  *   backward: with x' = q * scale, dx = dy * act'(x') and, where asked for, y' = act(x') (what the
  *             next layer's weight gradient reads, so that y need not be kept either).
- * act: WUBU_B200_ACT_*; slope: of the leaky ReLU (0 = ReLU), whose derivative at 0 is the slope.
+ * act: WUBU_B200_ACT_*; slope: of the leaky ReLU (0 = ReLU), whose derivative at 0 is the slope.  A value within
+ * half a step above 0 is kept as 0, so its derivative under ACT_LRELU is the slope's (about 0.5 % of
+ * normally distributed values: a tenth of the gradient's norm); ACT_LRELU_SIGN keeps it as one step and
+ * every derivative is that of x.
  * x, dy: `rows` rows of `cols` values, row strides in elements; y, q, dx, y_again: contiguous rows;
  * scale: [rows][ceil(cols / 128)].  y may be NULL (checkpoint only); dy and dx may both be NULL
  * (y_again only: with WUBU_B200_ACT_IDENTITY this restores x'). */
@@ -351,6 +354,7 @@ int wubu_b200_ops_sync(void* stream);
 #define WUBU_B200_ACT_LRELU 1
 #define WUBU_B200_ACT_GELU 2 /* x * Phi(x), the error-function form */
 #define WUBU_B200_ACT_SILU 3
+#define WUBU_B200_ACT_LRELU_SIGN 4 /* leaky ReLU; a positive value is kept as at least one step */
 int wubu_b200_act8_forward(int dtype, int act, float slope, const void* x, long long x_stride, void* y, signed char* q,
                            float* scale, long long rows, int cols, void* stream);
 int wubu_b200_act8_backward(int dtype, int act, float slope, const void* dy, long long dy_stride, const signed char* q,

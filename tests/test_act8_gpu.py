@@ -120,6 +120,22 @@ def test_gradient_against_differences():
     assert ((up - down).double() / (2 * h) - dx).abs().max() < 2e-4
 
 
+@pytest.mark.parametrize("C", [256, 250])
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+def test_lrelu_sign_keeps_every_derivative(C, dtype):
+    """Positive values are kept as at least one step: the derivative is that of x itself, exactly, and x' is off
+    by less than a step."""
+    g = torch.Generator().manual_seed(C)
+    x = torch.randn(60, C, generator=g).to(dtype).cuda()
+    dy = torch.randn(60, C, generator=g).to(dtype).cuda()
+    y, kept = tf.act8_forward(x, "lrelu_sign", slope=0.25)
+    dx, again = tf.act8_backward(dy, kept, recompute=True)
+    assert torch.equal(y, tf.act8_forward(x, "lrelu", slope=0.25)[0])
+    assert torch.equal(dx, torch.where(x > 0, dy, (dy.float() * 0.25).to(dtype)))
+    step = kept.scale.repeat_interleave(128, -1)[:, :C]
+    assert ((again.float() - y.float()).abs() <= 1.01 * step + U[dtype] * y.float().abs()).all()
+
+
 def test_empty():
     for shape in ((0, 64), (3, 0)):
         x = torch.empty(shape, device="cuda", dtype=torch.bfloat16)

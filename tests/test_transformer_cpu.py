@@ -1,0 +1,113 @@
+"""The transformer operators' checks that come before anything is launched: no GPU is needed.  The addresses
+are never followed."""
+import ctypes
+import struct
+
+import pytest
+import torch
+
+from wuburvc_b200 import transformer as tf
+
+OK, ARG, SHAPE, NOMEM = 0, -1, -3, -6
+A = 1 << 20  # an aligned address
+
+
+def act8(fn="forward", dtype=1, act=2, x=A, stride=64, y=A, q=A, scale=A, dx=A, rows=4, cols=64):
+    h = tf.L()
+    if fn == "forward":
+        return h.wubu_b200_act8_forward(dtype, act, 0.0, x, stride, y, q, scale, rows, cols, None)
+    return h.wubu_b200_act8_backward(dtype, act, 0.0, x, stride, q, scale, dx, y, rows, cols, None)
+
+
+def test_act8_refusals():
+    assert act8(rows=0) == OK and act8(cols=0) == OK and act8("backward", rows=0) == OK
+    for bad in (dict(dtype=3), dict(dtype=-1), dict(act=5), dict(act=-1), dict(rows=-1), dict(cols=-1), dict(q=None),
+                dict(scale=None), dict(x=None), dict(stride=63)):
+        assert act8(**bad) == ARG, bad
+    for bad in (dict(q=None), dict(scale=None), dict(x=None), dict(dx=None), dict(stride=10), dict(x=None, dx=None, y=None)):
+        assert act8("backward", **bad) == ARG, bad
+    assert act8(rows=1 << 40) == SHAPE
+
+
+RESNORM = ("dtype norm post gate items rows cols res_scale eps reserved x xs f fs weight bias post_weight post_bias gate_values "
+           "r h dr drs dh dhs dx df dgate dpost_weight dpost_bias dweight dbias ws n").split()
+
+
+def resnorm(fn, **kw):
+    v = dict.fromkeys(RESNORM, 0)
+    v.update(dtype=1, norm=1, items=2, rows=3, cols=64, res_scale=1.0, eps=1e-5, x=A, xs=64, f=A, fs=64, r=A, h=A, dh=A,
+             dhs=64, dx=A, df=A)
+    v.update(kw)
+    b = tf._RESNORM.pack(*(v[n] for n in RESNORM))
+    h = tf.L()
+    return h.wubu_b200_resnorm_workspace(b) if fn == "workspace" else getattr(h, "wubu_b200_resnorm_" + fn)(b, None)
+
+
+def test_resnorm_refusals():
+    assert resnorm("forward", items=0) == OK and resnorm("forward", rows=0) == OK
+    assert resnorm("workspace") > 0 and resnorm("workspace", items=0) == 0
+    for bad in (dict(dtype=5), dict(norm=3), dict(post=-1), dict(gate=3), dict(items=-1), dict(x=0), dict(f=0), dict(xs=63),
+                dict(gate=1), dict(eps=-1.0), dict(eps=float("nan"))):
+        assert resnorm("forward", **bad) == ARG, bad
+        assert resnorm("backward", **bad) == ARG, bad
+    for bad in (dict(cols=0), dict(cols=8193), dict(items=1 << 20, rows=1 << 20)):
+        assert resnorm("forward", **bad) == SHAPE and resnorm("workspace", **bad) == SHAPE
+    assert resnorm("forward", h=0) == ARG and resnorm("forward", norm=0) == ARG and resnorm("forward", norm=0, h=0, r=0) == ARG
+    for bad in (dict(norm=0), dict(dgate=A), dict(dpost_weight=A), dict(dweight=A), dict(dhs=8), dict(norm=0, dh=0, dweight=A)):
+        assert resnorm("backward", **bad) == ARG, bad
+    assert resnorm("backward", dweight=A, ws=A, n=16) == NOMEM
+
+
+ATTN = "dtype B Hq Hkv Tq Tk D causal window scale q_lens k_lens".split()
+
+
+def attn(fn, views=None, lse=A, ws=0, n=0, **kw):
+    v = dict(dtype=1, B=2, Hq=4, Hkv=2, Tq=10, Tk=12, D=64, causal=0, window=0, scale=0.0, q_lens=0, k_lens=0)
+    v.update(kw)
+    names = "q k v out dout dq dk dv".split()
+    w = {m: (A, v["D"] * 4 * 16, v["D"] * 4, v["D"]) for m in names}
+    w.update(views or {})
+    flat = [w[m] for m in names]
+    b = tf._ATTN.pack(*(v[m] for m in ATTN), *sum(flat[:4], ()), lse, *sum(flat[4:], ()), ws, n)
+    h = tf.L()
+    return h.wubu_b200_attn_workspace(b, 1) if fn == "workspace" else getattr(h, "wubu_b200_attn_" + fn)(b, None)
+
+
+def test_attention_refusals():
+    assert attn("forward", B=0) == OK and attn("backward", B=0) == OK and attn("forward", Tq=0, Tk=0) == OK
+    assert attn("workspace") > 0
+    for bad in (dict(dtype=0), dict(dtype=7), dict(B=-1), dict(Tq=-5), dict(window=-1), dict(scale=-1.0),
+                dict(scale=float("nan")), dict(scale=float("inf"))):
+        assert attn("forward", **bad) == ARG and attn("backward", **bad) == ARG, bad
+    for bad in (dict(D=0), dict(D=60), dict(D=136), dict(Hkv=3), dict(Hkv=0), dict(Hq=0), dict(B=70000), dict(Tk=1 << 29)):
+        assert attn("forward", **bad) == SHAPE and attn("workspace", **bad) == SHAPE, bad
+    for m in ("q", "k", "v", "out"):
+        for view in ((0, 4096, 256, 64), (A + 2, 4096, 256, 64), (A, 4096, 256, 60), (A, 4096, 0, 64), (A, -8, 256, 64),
+                     (A, 4096, 252, 64)):
+            assert attn("forward", views={m: view}) == ARG, (m, view)
+    for m in ("dout", "dq", "dk", "dv"):
+        assert attn("backward", views={m: (A + 8, 4096, 256, 64)}) == ARG
+    assert attn("forward", lse=0) == ARG
+    assert attn("backward", ws=A, n=8) == NOMEM and attn("backward") == ARG
+
+
+def test_structures_match_the_header(tmp_path):
+    src = tmp_path / "size.c"
+    src.write_text('#include "wuburvc_b200.h"\nint resnorm(void){return sizeof(WubuB200ResNorm);}\n'
+                   "int attn(void){return sizeof(WubuB200Attn);}\n")
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    so = str(tmp_path / "size.so")
+    subprocess.check_call(["gcc", "-shared", "-fPIC", "-I" + os.path.join(root, "include"), str(src), "-o", so])
+    lib = ctypes.CDLL(so)
+    assert lib.resnorm() == tf._RESNORM.size and lib.attn() == tf._ATTN.size
+    assert struct.calcsize("@P") == 8
+
+
+def test_binding_refuses_cpu_tensors():
+    x = torch.zeros(2, 3, 64)
+    for call in (lambda: tf.act8_forward(x), lambda: tf.resnorm_forward(x, x),
+                 lambda: tf.attention_forward(*(torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16),) * 3)):
+        with pytest.raises(ValueError):
+            call()

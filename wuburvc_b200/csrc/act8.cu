@@ -59,7 +59,8 @@ WB_DEV float normal_tail(float x, float& e) {
 
 template <int ACT>
 WB_DEV float act_value(float x, float slope) {
-  if (ACT == WUBU_B200_ACT_LRELU) return x > 0.f ? x : slope * x;
+  constexpr bool kLrelu = ACT == WUBU_B200_ACT_LRELU || ACT == WUBU_B200_ACT_LRELU_SIGN;
+  if (kLrelu) return x > 0.f ? x : slope * x;
   if (ACT == WUBU_B200_ACT_GELU) {
     float e;
     const float tail = normal_tail(x, e);
@@ -72,7 +73,8 @@ WB_DEV float act_value(float x, float slope) {
 // act(x) and act'(x)
 template <int ACT>
 WB_DEV void act_both(float x, float slope, float& y, float& d) {
-  if (ACT == WUBU_B200_ACT_LRELU) {
+  constexpr bool kLrelu = ACT == WUBU_B200_ACT_LRELU || ACT == WUBU_B200_ACT_LRELU_SIGN;
+  if (kLrelu) {
     d = x > 0.f ? 1.f : slope;
     y = x * d;
   } else if (ACT == WUBU_B200_ACT_GELU) {
@@ -126,8 +128,13 @@ WB_DEV void block_scale(uint32_t top, float& inv, float& scale) {
 }
 
 // round-to-even(x * inv) as an int8 in the low byte: adding 1.5 * 2^23 leaves the integer in the low bits of
-// the float
-WB_DEV uint32_t quantise(float x, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.f)); }
+// the float.  ACT_LRELU_SIGN: what is positive stays so.
+template <int ACT>
+WB_DEV uint32_t quantise(float x, float inv) {
+  float v = __fmul_rn(x, inv);
+  if (ACT == WUBU_B200_ACT_LRELU_SIGN && x > 0.f) v = fmaxf(v, 1.f);
+  return __float_as_uint(__fadd_rn(v, 12582912.f));
+}
 WB_DEV uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
@@ -168,7 +175,7 @@ __global__ void __launch_bounds__(kThreads) act8_forward_kernel(const Act8 a) {
     const long long at = row * a.cols + c0 + 64 * i;
     uint32_t q[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) q[k] = quantise(w[k], inv);
+    for (int k = 0; k < 8; ++k) q[k] = quantise<ACT>(w[k], inv);
     const uint2 packed = make_uint2(low_bytes(q[0], q[1], q[2], q[3]), low_bytes(q[4], q[5], q[6], q[7]));
     *reinterpret_cast<uint2*>(a.q + at) = bad ? make_uint2(0, 0) : packed;
     if (a.out) {
@@ -237,7 +244,7 @@ __global__ void __launch_bounds__(kThreads) act8_forward_any_kernel(const Act8 a
   for (int i = 0; i < 4; ++i) {
     if (c0 + 32 * i >= a.cols) continue;
     const long long at = row * a.cols + c0 + 32 * i;
-    a.q[at] = bad ? (signed char)0 : (signed char)quantise(v[i], inv);
+    a.q[at] = bad ? (signed char)0 : (signed char)quantise<ACT>(v[i], inv);
     if (a.out) static_cast<T*>(a.out)[at] = from_float<T>(act_value<ACT>(v[i], a.slope));
   }
 }
@@ -269,12 +276,13 @@ void with_act(int act, F f) {
   if (act == WUBU_B200_ACT_LRELU) f(std::integral_constant<int, WUBU_B200_ACT_LRELU>());
   else if (act == WUBU_B200_ACT_GELU) f(std::integral_constant<int, WUBU_B200_ACT_GELU>());
   else if (act == WUBU_B200_ACT_SILU) f(std::integral_constant<int, WUBU_B200_ACT_SILU>());
+  else if (act == WUBU_B200_ACT_LRELU_SIGN) f(std::integral_constant<int, WUBU_B200_ACT_LRELU_SIGN>());
   else f(std::integral_constant<int, WUBU_B200_ACT_IDENTITY>());
 }
 
 // Everything but the pointers; 1 = nothing to do.
 int check_act8(int dtype, int act, long long rows, int cols) {
-  if (!ops_dtype_ok(dtype) || act < WUBU_B200_ACT_IDENTITY || act > WUBU_B200_ACT_SILU) return WUBU_B200_ERR_ARG;
+  if (!ops_dtype_ok(dtype) || act < WUBU_B200_ACT_IDENTITY || act > WUBU_B200_ACT_LRELU_SIGN) return WUBU_B200_ERR_ARG;
   if (rows < 0 || cols < 0) return WUBU_B200_ERR_ARG;
   if (rows == 0 || cols == 0) return 1;
   const long long nblk = (cols + kBlock - 1) / kBlock;

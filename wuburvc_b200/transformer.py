@@ -5,7 +5,8 @@ besides their matrix products.
 * ``act8_forward`` / ``act8_backward``: an activation whose input is kept in 8 bits for the backward;
 * ``resnorm_forward`` / ``resnorm_backward``: the norms around a block, its gate and the residual scale;
 * ``attention_forward`` / ``attention_backward``: softmax attention, its gradient with the probabilities
-  recomputed from the log-sum-exp.
+  recomputed from the log-sum-exp;
+* ``attention``, ``resnorm``, ``feed_forward``: the same for torch's autograd.
 
 Calls enqueue on the current torch stream of the tensors' device and do not synchronise; outputs are new
 tensors.  A call that cannot be made raises (``ValueError`` for its arguments, ``RuntimeError`` for a
@@ -36,7 +37,7 @@ _SIGS = {
     "wubu_b200_attn_backward": (_ip, [ctypes.c_char_p, _vp]),
 }
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_ACTS = {"identity": 0, "lrelu": 1, "gelu": 2, "silu": 3}
+_ACTS = {"identity": 0, "lrelu": 1, "gelu": 2, "silu": 3, "lrelu_sign": 4}
 _NORMS = {None: 0, "layer": 1, "rms": 2}
 ACT8_BLOCK = 128
 _bound = None
@@ -151,7 +152,8 @@ class Kept8(NamedTuple):
 
 def act8_forward(x, act="gelu", slope=0.0, with_output=True):
     """``(act(x), kept)``; ``kept`` is what ``act8_backward`` reads in place of x.  ``act``: "lrelu"
-    (with ``slope``; 0 is the ReLU), "gelu", "silu" or "identity".  ``with_output=False`` only keeps x."""
+    (with ``slope``; 0 is the ReLU), "gelu", "silu" or "identity"; "lrelu_sign" is the leaky ReLU whose kept
+    positive values stay positive, so that its derivatives are exact.  ``with_output=False`` only keeps x."""
     d = _dtype(x, "act8_forward")
     if act not in _ACTS:
         raise ValueError(f"act8_forward: act is one of {sorted(_ACTS)}, got {act!r}")
@@ -415,3 +417,54 @@ class _Attention(torch.autograd.Function):
 def attention(q, k, v, **opts):
     """``attention_forward``'s out, differentiable by torch's autograd."""
     return _Attention.apply(q, k, v, opts)
+
+
+class _ResNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, f, weight, bias, post_weight, post_bias, gate, opts, keep_sum):
+        vec = dict(weight=weight, bias=bias, post_weight=post_weight, post_bias=post_bias, gate=gate)
+        ctx.save_for_backward(x, f, *vec.values())
+        ctx.opts = opts
+        ctx.set_materialize_grads(False)
+        return resnorm_forward(x, f, keep_sum=keep_sum, **vec, **opts)
+
+    @staticmethod
+    def backward(ctx, dr, dh):
+        x, f, *vec = ctx.saved_tensors
+        if dr is None and dh is None:
+            return (None,) * 9
+        names = ("weight", "bias", "post_weight", "post_bias", "gate")
+        g = resnorm_backward(dr, dh, x, f, **dict(zip(names, vec)), **ctx.opts)
+        cast = [None if v is None else g["d" + n].to(v.dtype) for n, v in zip(names, vec)]
+        return (g["dx"], g["df"], *cast, None, None)
+
+
+def resnorm(x, f, *, weight=None, bias=None, post_weight=None, post_bias=None, gate=None, keep_sum=True, **opts):
+    """``resnorm_forward``'s (r, h), differentiable by torch's autograd.  Only x and f are kept for the backward."""
+    return _ResNorm.apply(x, f, weight, bias, post_weight, post_bias, gate, opts, keep_sum)
+
+
+class _FeedForward(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w1, b1, w2, b2, act, slope):
+        y, kept = act8_forward(torch.nn.functional.linear(x, w1, b1), act, slope=slope)
+        ctx.save_for_backward(x, w1, w2, kept.q, kept.scale)
+        ctx.kept = (kept.act, kept.slope, kept.dtype, b1 is not None, b2 is not None)
+        return torch.nn.functional.linear(y, w2, b2)
+
+    @staticmethod
+    def backward(ctx, dout):
+        x, w1, w2, q, scale = ctx.saved_tensors
+        act, slope, dtype, has_b1, has_b2 = ctx.kept
+        du, y = act8_backward(dout @ w2, Kept8(q, scale, act, slope, dtype), recompute=True)
+        rows = lambda t: t.reshape(-1, t.shape[-1])  # noqa: E731
+        dw1, dw2 = rows(du).T @ rows(x), rows(dout).T @ rows(y)
+        db1 = rows(du).sum(0) if has_b1 else None
+        db2 = rows(dout).sum(0) if has_b2 else None
+        return du @ w1, dw1, db1, dw2, db2, None, None
+
+
+def feed_forward(x, w1, b1, w2, b2, act="gelu", slope=0.0):
+    """act(x w1^T + b1) w2^T + b2, differentiable.  Of its hidden layer the backward keeps the 8-bit form alone: the
+    activation's derivative and the input of w2's gradient are both formed from it."""
+    return _FeedForward.apply(x, w1, b1, w2, b2, act, slope)
