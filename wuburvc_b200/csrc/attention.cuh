@@ -254,6 +254,13 @@ WB_DEV void store_rows(uint8_t* stage, const uint32_t* w, T* row, long long stri
   }
   __syncwarp();
 }
+// Four floats from shared memory, in program order with the other volatile accesses (the compiler would load all
+// of a step's row values at its start and run out of registers).
+WB_DEV float4 lds4(const float* p) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(smem_u32(p)));
+  return v;
+}
 WB_DEV void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // A warp writes zeros over the tokens [from, 128) of a tile (what lies beyond an item's length may be

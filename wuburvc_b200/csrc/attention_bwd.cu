@@ -391,7 +391,7 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
           const int col0 = t * kTile + 32 * quarter;
           if (++t == t_end) t = t0;
           const uint32_t S = tmem + 256 * buf + lanes + 32 * quarter;
-          const float4* step_rows = reinterpret_cast<const float4*>(rows + sa * 2 * kTile + 32 * quarter);
+          const float* step_rows = rows + sa * 2 * kTile + 32 * quarter;
           if (KV) {
             if (ok) ok = bar_wait(&bar.a_full[sa], pa, p.err, ERR_WAIT_FULL, p.wait_ns);
             if (++sa == kA) {
@@ -411,7 +411,7 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
           for (int e = 0; e < 8; ++e) {
             uint64_t l01 = ll, l23 = ll;
             if (KV) {
-              const float4 v = step_rows[e];
+              const float4 v = lds4(step_rows + 4 * e);
               l01 = two(v.x, v.y);
               l23 = two(v.z, v.w);
             }
@@ -452,7 +452,7 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
               const float* xe = x + 16 * g + 4 * e;
               uint64_t d01 = dd, d23 = dd;
               if (KV) {
-                const float4 v = step_rows[kTile / 4 + 4 * g + e];
+                const float4 v = lds4(step_rows + kTile + 16 * g + 4 * e);
                 d01 = two(v.x, v.y);
                 d23 = two(v.z, v.w);
               }
@@ -496,32 +496,27 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
       for (int which = 0; which < 2; ++which) {
         if (!kv && which == 0) continue;
         const float sc = which ? ds_out : p_out;
-        float o[kCols];
-        if (k.steps > 0) {
-          const uint32_t at_ = (which ? tAcc1 : tAcc0) + lanes + d0;
-          if (kCols == 32) tmem_load<32>(at_, o);
-          else tmem_load16(at_, o);
-        }
-#pragma unroll
-        for (int e = 0; e < kCols; ++e) o[e] = live ? o[e] * sc : 0.f;
         const int tokens = kv ? a.Tk : a.Tq, H = kv ? a.Hkv : a.Hq, head = kv ? k.hk : k.hq;
-        if (SPLIT && (kv ? p.kv_splits : p.q_splits) > 1) {
-          float* part = (!kv ? p.part_dq : which ? p.part_dk : p.part_dv) +
-                        ((((long long)k.split * a.B + k.b) * H + head) * tokens + row) * a.D + d0;
+#pragma unroll 1
+        for (int d = d0; d < d0 + kCols; d += 16) {  // (one after the other: few registers)
+          float o[16];
+          if (k.steps > 0) tmem_load16((which ? tAcc1 : tAcc0) + lanes + d, o);
 #pragma unroll
-          for (int e = 0; e < kCols; e += 8)
-            if (row < tokens && d0 + e < a.D) store8(part + e, o + e);
-          __syncwarp();
-        } else {
-          const int r0 = k.own0 + (warp & 3) * 32;
-          const WubuB200View& view = !kv ? a.dq : which ? a.dk : a.dv;
-          T* out = at<T>(view, k.b, r0, head) + d0;
+          for (int e = 0; e < 16; ++e) o[e] = live ? o[e] * sc : 0.f;
+          if (SPLIT && (kv ? p.kv_splits : p.q_splits) > 1) {
+            float* part = (!kv ? p.part_dq : which ? p.part_dk : p.part_dv) +
+                          ((((long long)k.split * a.B + k.b) * H + head) * tokens + row) * a.D + d;
 #pragma unroll
-          for (int g = 0; g < kCols; g += 16) {
+            for (int e = 0; e < 16; e += 8)
+              if (row < tokens && d + e < a.D) store8(part + e, o + e);
+            __syncwarp();
+          } else {
+            const int r0 = k.own0 + (warp & 3) * 32;
+            const WubuB200View& view = !kv ? a.dq : which ? a.dk : a.dv;
             uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = pack2(o[g + 2 * e], o[g + 2 * e + 1], T());
-            store_rows<2>(stage + warp * 1024, w, out + g, view.token, tokens - r0, a.D - d0 - g);
+            for (int e = 0; e < 8; ++e) w[e] = pack2(o[2 * e], o[2 * e + 1], T());
+            store_rows<2>(stage + warp * 1024, w, at<T>(view, k.b, r0, head) + d, view.token, tokens - r0, a.D - d);
           }
         }
       }
