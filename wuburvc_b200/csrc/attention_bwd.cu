@@ -14,7 +14,8 @@
 // Sixteen warps do the exponentials, four to a row quadrant, 32 columns a thread; one warp loads, one
 // issues.  A CTA an SM works through the items of both roles, loading the next one's tiles behind the last
 // one's steps; where one item would outlast the rest, its steps are split and float32 parts joined.  A step's products and its elementwise halves alternate:
-//   keys' role:     tensor  dV(n) S(n+1) | dK(n) dP(n+1)      warps  dS(n) | P(n+1)
+//   keys' role:     tensor  dV(n) S(n+1) | dK(n) dP(n+1)      warps  dS(n) | P(n+1)        at 128 values a row
+//                           dV(n) | dK(n) dP(n+1) S(n+2)             dS(n) | P(n+1)        up to 64
 //   queries' role:  tensor  dQ(n) dP(n+1) S(n+2)              warps  P(n+1) dS(n+1)
 //
 // fp16 has few small numbers and a low ceiling, so its P is scaled by 2^14 (P <= 1) and its dS by the
@@ -150,6 +151,9 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
   constexpr int kBoxes = DP / 64;
   constexpr uint32_t kTileBytes = kBoxes * kBox;
   constexpr int kA = kStagesA<DP>;
+  // Up to 64 values a row two S fit beside the accumulators in the keys' role too, and S(n+2) is issued behind step
+  // n's last product; at 128 its single S has to wait for dV(n), which reads P from it.
+  constexpr bool kTwoS = DP == 64;
   constexpr float kShift = BwdShift<T>::value;
   constexpr int kBf16 = std::is_same<T, bf16>::value;
   extern __shared__ uint8_t smem_raw[];
@@ -196,8 +200,9 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  // columns: S at 0 (queries' role: every second step's at 256), dP at 128, dV at 256, dK or dQ at 384
-  const uint32_t tDP = tmem + 128, tAcc0 = tmem + 256, tAcc1 = tmem + 384;
+  // columns: S at 0 (every second step's at 256, but for the keys' role at 128 values), dP at 128; dV at 384 and dK or
+  // dQ at 448, at 128 values at 256 and 384
+  const uint32_t tDP = tmem + 128, tAcc0 = tmem + (kTwoS ? 384 : 256), tAcc1 = tmem + (kTwoS ? 448 : 384);
 
   if (warp >= kProducer) {
     regs_dec<64>();
@@ -271,6 +276,7 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
         const bool kv = k.kv;
         if (ok) ok = bar_wait(&bar.res_full, items & 1, p.err, ERR_WAIT_FULL, p.wait_ns);
         ++items;
+        const bool two_s = kTwoS || !kv;
         int ta = k.t, tb = k.t, unused = 0;  // tiles of the next S and dP
         // step n's tile in a ring, its rows beyond the item's length cleared
         auto clear = [&](uint8_t* tile, int tt) {
@@ -278,7 +284,7 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
           if (ok && valid < kTile) zero_rows(tile, max(valid, 0), kBoxes);
         };
         auto issue_s = [&](int i) {
-          const int n = n0 + i, sa = n % kA, buf = kv ? 0 : i & 1;
+          const int n = n0 + i, sa = n % kA, buf = two_s ? i & 1 : 0;
           if (ok) ok = bar_wait(&bar.a_full[sa], (n / kA) & 1, p.err, ERR_WAIT_FULL, p.wait_ns);
           clear(ra + sa * kTileBytes, ta);
           k.advance(ta, unused);
@@ -307,9 +313,9 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
         };
         issue_s(0);
         issue_dp(0);
-        if (!kv && k.steps > 1) {
-          // the second buffer of S may still be the last item's dV
-          if (ok && all) ok = bar_wait(&bar.acc_read, (all - 1) & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
+        if (two_s && k.steps > 1) {
+          // at 128 values the second S may still be the last item's dV
+          if (!kTwoS && ok && all) ok = bar_wait(&bar.acc_read, (all - 1) & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
           tc_fence_after();
           issue_s(1);
         }
@@ -320,10 +326,10 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
             ++p_count;
             tc_fence_after();
             if (ok) {
-              issue_acc(tAcc0, tmem, rb + sb * kTileBytes, i);
+              issue_acc(tAcc0, tmem + (two_s ? 256 * (i & 1) : 0), rb + sb * kTileBytes, i);
               umma_commit_warp(&bar.b_empty[sb]);
             }
-            if (i + 1 < k.steps) issue_s(i + 1);
+            if (!two_s && i + 1 < k.steps) issue_s(i + 1);
           }
           if (ok) ok = bar_wait(&bar.ds_ready, n & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
           tc_fence_after();
@@ -333,7 +339,7 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
             if (i == k.steps - 1) umma_commit_warp(&bar.acc_full);
           }
           if (i + 1 < k.steps) issue_dp(i + 1);
-          if (!kv && i + 2 < k.steps) issue_s(i + 2);
+          if (two_s && i + 2 < k.steps) issue_s(i + 2);
         }
         n0 += k.steps;
       }
@@ -386,7 +392,7 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
         int sa = n0 % kA;
         uint32_t pa = (n0 / kA) & 1;
         for (int i = 0; i < steps; ++i) {
-          const int buf = KV ? 0 : i & 1;
+          const int buf = KV && !kTwoS ? 0 : i & 1;
           const bool masked = t < whole0 || t >= whole1;
           const int col0 = t * kTile + 32 * quarter;
           if (++t == t_end) t = t0;
