@@ -60,8 +60,11 @@ struct BwdWork {
   int b, hk, hq, own0, split;
   int t0, per_head;      // the other side's first tile and their count, for each head
   int steps, t, h;       // of this part: steps, and where they start
+  bool none;             // no item: the work is done
+  BwdWork() = default;
   WB_DEV BwdWork(const AttnParams& p, int id, int kv_work) {
     const WubuB200Attn& a = p.a;
+    none = false;
     kv = id < kv_work;
     unsigned r = kv ? id : id - kv_work;
     const unsigned heads = kv ? a.Hkv : a.Hq, splits = kv ? p.kv_splits : p.q_splits;
@@ -126,25 +129,29 @@ WB_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar)
       : "memory");
 }
 
-// SPLIT: in one role at least the steps of an item are split.
 // The CTAs take items in order as they come free (the lengths and causal order make items unequal): the first by
-// their number, the rest from a counter that the kernel before has cleared.  The loading warp draws and
-// hands the number to the other warps.  Which CTA works on an item does not change its result.
+// their number, the rest from a counter that the kernel before has cleared.  The loading warp draws, works
+// the item out (divisions and the item's lengths: about a thousand cycles, behind the last item's steps) and hands
+// it to the other warps.  Which CTA works on an item does not change its result.
 struct Items {
   Barriers& bar;
-  volatile int* slots;
+  const BwdWork* slots;
   int n;  // taken so far
-  WB_DEV bool take(int& id, const AttnParams& p, int work) {
+  WB_DEV bool take(BwdWork& k, const AttnParams& p) {
     const int s = n & 1;
     const bool ok = bar_wait(&bar.item_full[s], (n >> 1) & 1, p.err, ERR_WAIT_FULL, p.wait_ns);
-    id = ok ? slots[s] : work;
+    k = slots[s];
+    if (!ok) k.none = true;
+    return !k.none;
+  }
+  WB_DEV void done() {  // with the item as it lies in the slot
     __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(&bar.item_empty[s]);
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&bar.item_empty[n & 1]);
     ++n;
-    return id < work;
   }
 };
 
+// SPLIT: in one role at least the steps of an item are split.
 template <typename T, int DP, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_constant__ AttnParams p, int kv_work, int work) {
@@ -166,7 +173,7 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
   // keys' role: the log-sum-exp and row sum of a step's 128 queries, with the first ring's tiles
   float* rows = reinterpret_cast<float*>(stage + kProducer * 1024);
   __shared__ Barriers bar;
-  __shared__ int item_slots[2];
+  __shared__ BwdWork item_slots[2];
   __shared__ uint32_t tmem_slot;
 
   const WubuB200Attn& a = p.a;
@@ -212,16 +219,17 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
       int n = 0, items = 0, drawn = 0;  // steps, items with steps, and all items so far
       int next = blockIdx.x;
       for (;;) {
-        int id = __shfl_sync(0xffffffffu, next, 0);
+        const int id = __shfl_sync(0xffffffffu, next, 0);
         if (ok && drawn >= 2) ok = bar_wait(&bar.item_empty[drawn & 1], ((drawn >> 1) & 1) ^ 1u, p.err, ERR_WAIT_EMPTY, p.wait_ns);
-        if (!ok) id = work;
+        const bool none = !ok || id >= work;
+        BwdWork k(p, none ? 0 : id, kv_work);
+        k.none = none;
         if (lane == 0) {
-          item_slots[drawn & 1] = id;
+          item_slots[drawn & 1] = k;
           mbar_arrive(&bar.item_full[drawn & 1]);
         }
         __syncwarp();
-        if (id >= work) break;
-        const BwdWork k(p, id, kv_work);
+        if (none) break;
         if (drawn++ == 0) griddep_wait();  // the counter, the row sums and log-sum-exps come from the kernel before
         // (drawn here, looked at when the item's loads are out)
         next = lane == 0 ? (int)gridDim.x + (int)atomicAdd(p.counter, 1u) : 0;
@@ -270,8 +278,8 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
       int n0 = 0, items = 0, p_count = 0;
       int all = 0;  // items so far, those without steps too
       Items take{bar, item_slots, 0};
-      for (int id; take.take(id, p, work); ++all) {
-        const BwdWork k(p, id, kv_work);
+      for (BwdWork k; take.take(k, p); ++all) {
+        take.done();
         if (k.steps == 0) continue;
         const bool kv = k.kv;
         if (ok) ok = bar_wait(&bar.res_full, items & 1, p.err, ERR_WAIT_FULL, p.wait_ns);
@@ -358,13 +366,14 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
     uint32_t s_phase[2] = {0, 0};  // of the two buffers of S
     griddep_wait();                // the queries' role reads row sums and log-sum-exps itself
     Items take{bar, item_slots, 0};
-    for (int id; take.take(id, p, work);) {
+    for (;;) {
       bool kv;
       int steps, t, t0, t_end;             // steps; the next step's tile, and the range that it runs through
       int lo, hi, whole0, whole1;          // the row's range, and the tiles that need no mask
       float l2 = 0.f, delta = 0.f, f = 1.f;  // queries' role: the row's values; the scale of P 2^shift (dP - D)
       {
-        const BwdWork k(p, id, kv_work);
+        BwdWork k;
+        if (!take.take(k, p)) break;
         kv = k.kv;
         steps = k.steps;
         t = k.t;
@@ -484,8 +493,8 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
       };
       if (kv) run(std::true_type());
       else run(std::false_type());
-      asm volatile("" : "+r"(id));  // (formed again rather than held in registers over the steps)
-      const BwdWork k(p, id, kv_work);
+      const BwdWork k = item_slots[take.n & 1];  // (read again rather than held in registers over the steps)
+      take.done();
       n0 += k.steps;
       if (k.steps > 0) {
         if (ok) ok = bar_wait(&bar.acc_full, items & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
