@@ -22,7 +22,7 @@ namespace wb {
 namespace {
 
 // Eight softmax warps (a row of 128 scores in registers each thread), and a warpgroup of which one warp
-// loads and one issues the products.  384 threads are launched with 168 registers; the split 256 x 216 +
+// loads and two issue the products.  384 threads are launched with 168 registers; the split 256 x 216 +
 // 128 x 72 is the same 64512.
 constexpr int kProducer = 8, kMma = 9, kThreads = 384;  // kMma + s issues stream s
 
@@ -45,8 +45,11 @@ struct FwdWork {
   int b, h, split;
   int q0[2], t0[2], t1[2];  // per stream: first query, key tiles [t0, t1)
   int u0, u1;               // the tiles that either stream meets
+  bool none;                // no item: the work is done
+  FwdWork() = default;
   WB_DEV FwdWork(const AttnParams& p, int id) {
     const WubuB200Attn& a = p.a;
+    none = false;
     const unsigned t = (unsigned)id / (unsigned)a.Hq;
     h = id - t * a.Hq;
     unsigned r = t / (unsigned)a.B;
@@ -104,7 +107,8 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
   uint8_t* vt = kt + kStages * kTileBytes;
   uint8_t* stage = vt + kStages * kTileBytes;  // 2 KB a softmax warp
   // per stream: S complete; S read (kApart); the halves of P written; the product that read P done
-  __shared__ uint64_t q_full[2], q_empty[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2],
+  __shared__ FwdWork items[2];  // worked out by the loading warp (about a thousand cycles), behind the last item
+  __shared__ uint64_t item_full[2], item_empty[2], q_full[2], q_empty[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2],
       s_read[2], p_ready[2][2], pv_done[2], turn[2], mma_done[2];
   __shared__ uint32_t tmem_slot;
 
@@ -114,6 +118,8 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], kProducer + 2);
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
@@ -136,6 +142,14 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  // item n's slot: false at the end of the work
+  auto take = [&](int n) {
+    return bar_wait(&item_full[n & 1], (n >> 1) & 1, p.err, ERR_WAIT_FULL, p.wait_ns) && !items[n & 1].none;
+  };
+  auto done = [&](int n) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_empty[n & 1]);
+  };
   // columns: S at 0 and 128; apart, P at 256 and 320 and O at 384 and 448; else P over S and O at 256 and 384
   auto col_p = [&](int s) { return tmem + (kApart ? 256 + 64 * s : 128 * s); };
   auto col_o = [&](int s) { return tmem + (kApart ? 384 + 64 * s : 256 + 128 * s); };
@@ -146,8 +160,18 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
       bool ok = true;
       FillTrack fq, fk, fv;
       int n = 0, nq[2] = {0, 0};  // tiles loaded so far
-      for (AttnRounds r(work); r.more(); r.advance()) {
-        const FwdWork k(p, r.next);
+      int count = 0;
+      for (AttnRounds r(work);; r.advance(), ++count) {
+        if (ok && count >= 2) ok = bar_wait(&item_empty[count & 1], ((count >> 1) & 1) ^ 1u, p.err, ERR_WAIT_EMPTY, p.wait_ns);
+        const bool none = !ok || !r.more();
+        FwdWork k(p, none ? 0 : r.next);
+        k.none = none;
+        if (lane == 0) {
+          items[count & 1] = k;
+          mbar_arrive(&item_full[count & 1]);
+        }
+        __syncwarp();
+        if (none) break;
         const int hk = k.h / p.group;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -191,8 +215,9 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
       bool ok = true;
       uint32_t ph = 0;     // of the stream's tiles
       int n0 = 0, nq = 0;  // tiles in the rings before this item; the stream's query tiles
-      for (AttnRounds r(work); r.more(); r.advance()) {
-        const FwdWork k(p, r.next);
+      for (int count = 0; take(count); ++count) {
+        const FwdWork k = items[count & 1];
+        done(count);
         const int st0 = s ? k.t0[1] : k.t0[0], st1 = s ? k.t1[1] : k.t1[0], u0 = k.u0, u1 = k.u1;
         // the scores against key tile j, or a pass by a tile that the stream does not meet
         auto issue_s = [&](int j) {
@@ -268,8 +293,8 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
       if (s == 0 && ok && g_turn) ok = bar_wait(&turn[1], (g_turn - 1) & 1u, p.err, ERR_WAIT_ACC, p.wait_ns);
       ++g_turn;
     };
-    for (AttnRounds r(work); r.more(); r.advance()) {
-      const FwdWork next(p, r.next);
+    for (int count = 0; take(count); ++count) {
+      const FwdWork& next = items[count & 1];
       const int n_s0 = next.t1[0] - next.t0[0], n_s1 = next.t1[1] - next.t0[1];
       const bool turns = !kApart && n_s0 > 0 && n_s1 > 0;
       const bool empty_turn = turns && (s ? n_s1 < n_s0 : n_s0 < n_s1);
@@ -408,6 +433,7 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
           store_rows<4>(stage + warp * 2048, w, out + d0, a.out.token, a.Tq - r0, a.D - d0);
         }
       }
+      done(count);
       tc_fence_before();  // O is read before the next item's first product may be issued
     }
   }
