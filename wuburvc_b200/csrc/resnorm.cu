@@ -342,6 +342,7 @@ struct ColumnSums {
 };
 __global__ void __launch_bounds__(kReduceCols* kReduceRuns) resnorm_sums_kernel(const ColumnSums s, int cols) {
   __shared__ float run[kReduceRuns][kReduceCols];
+  griddep_wait();
   const int q = min((int)blockIdx.y, s.count), item = blockIdx.y - q;
   const int c = blockIdx.x * kReduceCols + threadIdx.x;
   const int n = s.n[q], per = (n + kReduceRuns - 1) / kReduceRuns;
@@ -498,9 +499,8 @@ int wubu_b200_resnorm_backward(const WubuB200ResNorm* p, void* stream) {
     s.count = k++;
     sums_y += by_item ? (int)a.items : 1;
   }
-  resnorm_sums_kernel<<<dim3((a.cols + kReduceCols - 1) / kReduceCols, sums_y), dim3(kReduceCols, kReduceRuns), 0, st>>>(
-      s, a.cols);
-  return ops_launched("resnorm_sums");
+  return ops_launch_after(resnorm_sums_kernel, dim3((a.cols + kReduceCols - 1) / kReduceCols, sums_y),
+                          dim3(kReduceCols, kReduceRuns), 0, st, "resnorm_sums", s, a.cols);
 }
 
 }  // extern "C"
