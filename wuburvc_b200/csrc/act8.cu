@@ -43,53 +43,72 @@ WB_DEV float fast_rcp(float x) {
   return y;
 }
 
-// Phi(-|x|) and e^(-x^2/2): the first is the second times a polynomial in t = 1 / (1 + p |x| / sqrt 2) (Abramowitz
-// and Stegun, Handbook of Mathematical Functions, 7.1.26, halved; absolute error below 1e-7).
-// Straight-line code with one exponential and one reciprocal: a library erff in two ranges with expf
-// beside it took twice the time of the memory traffic.
-WB_DEV float normal_tail(float x, float& e) {
-  const float t = fast_rcp(fmaf(0.3275911f * 0.70710678118654752f, fabsf(x), 1.f));
-  e = fast_ex2(x * x * -0.72134752044448170f);
-  float s = fmaf(0.5f * 1.061405429f, t, -0.5f * 1.453152027f);
-  s = fmaf(s, t, 0.5f * 1.421413741f);
-  s = fmaf(s, t, -0.5f * 0.284496736f);
-  s = fmaf(s, t, 0.5f * 0.254829592f);
-  return s * t * e;
+WB_DEV uint64_t both(float v) { return two(v, v); }
+WB_DEV uint64_t abs2(uint64_t x) { return x & 0x7FFFFFFF7FFFFFFFull; }
+WB_DEV uint64_t rcp2(uint64_t x) {
+  float a, b;
+  each(x, a, b);
+  return two(fast_rcp(a), fast_rcp(b));
+}
+WB_DEV uint64_t ex22(uint64_t x) {
+  float a, b;
+  each(x, a, b);
+  return two(fast_ex2(a), fast_ex2(b));
+}
+
+// Phi(-|x|) and e^(-x^2/2) of two values: the first is the second times a polynomial in t = 1 / (1 + p |x| / sqrt 2)
+// (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26, halved; absolute error below 1e-7).
+// Straight-line code with one exponential and one reciprocal a value: a library erff in two ranges with expf
+// beside it took twice the time of the memory traffic, and one value at a time these kernels were still
+// bound by instruction issue (31 a value).
+WB_DEV uint64_t normal_tail2(uint64_t x, uint64_t& e) {
+  const uint64_t t = rcp2(fma2(both(0.3275911f * 0.70710678118654752f), abs2(x), both(1.f)));
+  e = ex22(mul2(mul2(x, x), both(-0.72134752044448170f)));
+  uint64_t s = fma2(both(0.5f * 1.061405429f), t, both(-0.5f * 1.453152027f));
+  s = fma2(s, t, both(0.5f * 1.421413741f));
+  s = fma2(s, t, both(-0.5f * 0.284496736f));
+  s = fma2(s, t, both(0.5f * 0.254829592f));
+  return mul2(mul2(s, t), e);
 }
 
 template <int ACT>
-WB_DEV float act_value(float x, float slope) {
-  constexpr bool kLrelu = ACT == WUBU_B200_ACT_LRELU || ACT == WUBU_B200_ACT_LRELU_SIGN;
-  if (kLrelu) return x > 0.f ? x : slope * x;
+WB_DEV uint64_t act_value2(uint64_t x, float slope) {
+  float a, b;
+  each(x, a, b);
+  if (ACT == WUBU_B200_ACT_LRELU || ACT == WUBU_B200_ACT_LRELU_SIGN)
+    return two(a > 0.f ? a : slope * a, b > 0.f ? b : slope * b);
   if (ACT == WUBU_B200_ACT_GELU) {
-    float e;
-    const float tail = normal_tail(x, e);
-    // x Phi(x) = max(x, 0) - |x| Phi(-|x|), whose second term is 0 from |x| = 64 on; NaN stays NaN
-    return fmaf(-fminf(fabsf(x), 64.f), tail, x > 0.f ? x : x * 0.f);
+    // x Phi(x) = max(x, 0) - |x| Phi(-|x|), whose second term is 0 from |x| = 64 on (so that infinity stays)
+    uint64_t e;
+    const uint64_t tail = normal_tail2(x, e);
+    return fma2(two(-fminf(fabsf(a), 64.f), -fminf(fabsf(b), 64.f)), tail, two(fmaxf(a, 0.f), fmaxf(b, 0.f)));
   }
-  if (ACT == WUBU_B200_ACT_SILU) return x * fast_rcp(1.f + fast_ex2(x * -1.4426950408889634f));
+  if (ACT == WUBU_B200_ACT_SILU) return mul2(x, rcp2(add2(both(1.f), ex22(mul2(x, both(-1.4426950408889634f))))));
   return x;
 }
 // act(x) and act'(x)
 template <int ACT>
-WB_DEV void act_both(float x, float slope, float& y, float& d) {
-  constexpr bool kLrelu = ACT == WUBU_B200_ACT_LRELU || ACT == WUBU_B200_ACT_LRELU_SIGN;
-  if (kLrelu) {
-    d = x > 0.f ? 1.f : slope;
-    y = x * d;
+WB_DEV void act_both2(uint64_t x, float slope, uint64_t& y, uint64_t& d) {
+  if (ACT == WUBU_B200_ACT_LRELU || ACT == WUBU_B200_ACT_LRELU_SIGN) {
+    float a, b;
+    each(x, a, b);
+    d = two(a > 0.f ? 1.f : slope, b > 0.f ? 1.f : slope);
+    y = mul2(x, d);
   } else if (ACT == WUBU_B200_ACT_GELU) {
-    float e;
-    const float tail = normal_tail(x, e);
-    const float cdf = 0.5f + copysignf(0.5f - tail, x);
-    y = x * cdf;
-    d = fmaf(x * 0.39894228040143268f, e, cdf);
+    uint64_t e;
+    const uint64_t tail = normal_tail2(x, e);
+    // Phi(x) = 1/2 + (1/2 - Phi(-|x|)) with x's sign
+    const uint64_t h = fma2(tail, both(-1.f), both(0.5f));
+    const uint64_t cdf = add2(both(0.5f), abs2(h) | (x & 0x8000000080000000ull));
+    y = mul2(x, cdf);
+    d = fma2(mul2(x, both(0.39894228040143268f)), e, cdf);
   } else if (ACT == WUBU_B200_ACT_SILU) {
-    const float t = fast_rcp(1.f + fast_ex2(x * -1.4426950408889634f));
-    y = x * t;
-    d = fmaf(y, 1.f - t, t);
+    const uint64_t t = rcp2(add2(both(1.f), ex22(mul2(x, both(-1.4426950408889634f)))));
+    y = mul2(x, t);
+    d = fma2(y, fma2(t, both(-1.f), both(1.f)), t);
   } else {
     y = x;
-    d = 1.f;
+    d = both(1.f);
   }
 }
 
@@ -129,6 +148,7 @@ WB_DEV void block_scale(uint32_t top, float& inv, float& scale) {
 
 // round-to-even(x * inv) as an int8 in the low byte: adding 1.5 * 2^23 leaves the integer in the low bits of
 // the float.  ACT_LRELU_SIGN: what is positive stays so.
+// One value at a time: the assembler joins a product and a sum of two values into one rounding.
 template <int ACT>
 WB_DEV uint32_t quantise(float x, float inv) {
   float v = __fmul_rn(x, inv);
@@ -180,7 +200,7 @@ __global__ void __launch_bounds__(kThreads) act8_forward_kernel(const Act8 a) {
     *reinterpret_cast<uint2*>(a.q + at) = bad ? make_uint2(0, 0) : packed;
     if (a.out) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) w[k] = act_value<ACT>(w[k], a.slope);
+      for (int k = 0; k < 8; k += 2) each(act_value2<ACT>(two(w[k], w[k + 1]), a.slope), w[k], w[k + 1]);
       store8(static_cast<T*>(a.out) + at, w);
     }
   }
@@ -209,10 +229,13 @@ __global__ void __launch_bounds__(kThreads) act8_backward_kernel(const Act8 a) {
     float y[8];
     const uint32_t lo = q[i].x ^ 0x80808080u, hi = q[i].y ^ 0x80808080u;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      float d;
-      act_both<ACT>(dequantise(k < 4 ? lo : hi, k & 3) * scale, a.slope, y[k], d);
-      g[i][k] *= d;
+    for (int k = 0; k < 8; k += 2) {
+      const uint32_t w = k < 4 ? lo : hi;
+      const uint64_t x = mul2(two(dequantise(w, k & 3), dequantise(w, (k & 3) + 1)), both(scale));
+      uint64_t yy, d;
+      act_both2<ACT>(x, a.slope, yy, d);
+      each(yy, y[k], y[k + 1]);
+      each(mul2(two(g[i][k], g[i][k + 1]), d), g[i][k], g[i][k + 1]);
     }
     if (a.out) store8(static_cast<T*>(a.out) + at + 64 * i, g[i]);
     if (a.again) store8(static_cast<T*>(a.again) + at + 64 * i, y);
@@ -240,12 +263,20 @@ __global__ void __launch_bounds__(kThreads) act8_forward_any_kernel(const Act8 a
   block_scale(top, inv, scale);
   if (lane == 0) a.scale[blk] = scale;
   const bool bad = top >= 0x7F800000u;
+  uint32_t q[4];
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {  // (the same operations as above, value for value)
+    q[i] = quantise<ACT>(v[i], inv);
+    q[i + 1] = quantise<ACT>(v[i + 1], inv);
+    each(act_value2<ACT>(two(v[i], v[i + 1]), a.slope), y[i], y[i + 1]);
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (c0 + 32 * i >= a.cols) continue;
     const long long at = row * a.cols + c0 + 32 * i;
-    a.q[at] = bad ? (signed char)0 : (signed char)quantise<ACT>(v[i], inv);
-    if (a.out) static_cast<T*>(a.out)[at] = from_float<T>(act_value<ACT>(v[i], a.slope));
+    a.q[at] = bad ? (signed char)0 : (signed char)q[i];
+    if (a.out) static_cast<T*>(a.out)[at] = from_float<T>(y[i]);
   }
 }
 
@@ -262,8 +293,11 @@ __global__ void __launch_bounds__(kThreads) act8_backward_any_kernel(const Act8 
     const int c = c0 + 32 * i;
     if (c >= a.cols) continue;
     const long long at = row * a.cols + c;
-    float y, d;
-    act_both<ACT>((float)a.q[at] * scale, a.slope, y, d);
+    uint64_t yy, dd;
+    float y, d, unused;
+    act_both2<ACT>(two((float)a.q[at] * scale, 0.f), a.slope, yy, dd);
+    each(yy, y, unused);
+    each(dd, d, unused);
     if (a.out)
       static_cast<T*>(a.out)[at] =
           from_float<T>(to_float(static_cast<const T*>(a.in)[row * a.in_stride + c]) * d);
