@@ -118,6 +118,20 @@ def test_shapes_and_masks(shape, mask, dtype):
     check(*make(*shape, dtype, seed=sum(shape)), **MASKS[mask])
 
 
+@pytest.mark.parametrize("shape", [(8, 12, 12, 300, 300, 64), (8, 8, 4, 260, 389, 128), (16, 6, 6, 400, 400, 96)], ids=str)
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+def test_many_heads(shape, dtype):
+    """More items than SMs, several tiles each: every CTA takes several, and no item is split."""
+    check(*make(*shape, dtype, seed=7), causal=True)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_sequences(D):
+    """Many tiles an item: the rings go round, the running maximum and the sums span 20 tiles."""
+    check(*make(1, 4, 1, 2500, 2500, D, torch.bfloat16, seed=D), causal=True)
+    check(*make(1, 2, 2, 3, 5000, D, torch.float16, seed=D))
+
+
 @pytest.mark.parametrize("mask", list(MASKS))
 @pytest.mark.parametrize("T,D", [(300, 64), (130, 96), (70, 128)])
 @pytest.mark.parametrize("dtype", list(U), ids=str)

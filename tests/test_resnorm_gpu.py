@@ -107,6 +107,17 @@ def test_every_form(norm, post, gate):
         check((2, 21, 96), torch.float32, norm, post, gate, use_dh=False)
 
 
+def test_rows_without_items():
+    """[rows, cols]: every row is an item, which takes no more workspace than the same rows in one item."""
+    for gate in (None, "column", "item"):
+        check((70, 96), torch.float32, "layer", "rms", gate)
+    x = torch.randn(40000, 64, device="cuda").to(torch.bfloat16)
+    w = torch.rand(64, device="cuda")
+    flat = tf.resnorm_backward(x, x, x, x, weight=w)
+    whole = tf.resnorm_backward(*(x[None],) * 4, weight=w)
+    assert torch.equal(flat["dx"], whole["dx"][0]) and torch.equal(flat["dweight"], whole["dweight"])
+
+
 def test_strided_rows():
     big = torch.randn(4, 10, 3 * 64, device="cuda").to(torch.bfloat16)
     x, f = big[..., :64], big[..., 64:128]

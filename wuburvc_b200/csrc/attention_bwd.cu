@@ -13,7 +13,8 @@
 // (rows are keys), so that P^T and dS^T are written over them as the A operands of the next products.
 // Sixteen warps do the exponentials, four to a row quadrant, 32 columns a thread; one warp loads, one
 // issues.  A CTA an SM works through the items of both roles, loading the next one's tiles behind the last
-// one's steps; where one item would outlast the rest, its steps are split and float32 parts joined.  A step's products and its elementwise halves alternate:
+// one's steps; where one item would outlast the rest, its steps are split and float32 parts joined.  A
+// step's products and its elementwise halves alternate:
 //   keys' role:     tensor  dV(n) S(n+1) | dK(n) dP(n+1)      warps  dS(n) | P(n+1)        at 128 values a row
 //                           dV(n) | dK(n) dP(n+1) S(n+2)             dS(n) | P(n+1)        up to 64
 //   queries' role:  tensor  dQ(n) dP(n+1) S(n+2)              warps  P(n+1) dS(n+1)

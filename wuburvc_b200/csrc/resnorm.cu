@@ -384,6 +384,17 @@ int check_resnorm(const WubuB200ResNorm* a) {
 
 bool vec_ok(const WubuB200ResNorm& a, const void* p, long long stride) { return aligned16(p) && stride % 8 == 0; }
 
+// Items matter to their gates alone: without such gates the rows are one item's, and the row ranges (and
+// the partial sums, one row of them to a range) do not depend on how the rows were numbered.
+WubuB200ResNorm as_ranges(const WubuB200ResNorm& in) {
+  WubuB200ResNorm a = in;
+  if (a.gate != WUBU_B200_GATE_ITEM) {
+    a.rows_per_item *= a.items;
+    a.items = 1;
+  }
+  return a;
+}
+
 // threads a row (a multiple of 32), rows at a time (a barrier each: at most 15)
 dim3 group_of(int cols) {
   const int G = (((cols + 7) / 8) + 31) / 32 * 32;
@@ -418,7 +429,7 @@ extern "C" {
 int wubu_b200_resnorm_forward(const WubuB200ResNorm* p, void* stream) {
   const int rc = check_resnorm(p);
   if (rc != WUBU_B200_OK) return rc == 1 ? WUBU_B200_OK : rc;
-  WubuB200ResNorm a = *p;
+  WubuB200ResNorm a = as_ranges(*p);
   if (!a.norm != !a.h || (!a.r && !a.h)) return WUBU_B200_ERR_ARG;
   const long long rows = a.items * a.rows_per_item;
   if (rows == 1) a.x_stride = a.f_stride = 0;
@@ -440,14 +451,14 @@ int wubu_b200_resnorm_forward(const WubuB200ResNorm* p, void* stream) {
 long long wubu_b200_resnorm_workspace(const WubuB200ResNorm* a) {
   const int rc = check_resnorm(a);
   if (rc != WUBU_B200_OK) return rc == 1 ? 0 : rc;
-  return grid_of(*a, group_of(a->cols), 1).blocks * kVectors * a->cols * (long long)sizeof(float);
+  return grid_of(as_ranges(*a), group_of(a->cols), 1).blocks * kVectors * a->cols * (long long)sizeof(float);
 }
 
 int wubu_b200_resnorm_backward(const WubuB200ResNorm* p, void* stream) {
   int rc = check_resnorm(p);
   cudaStream_t st = (cudaStream_t)stream;
   if (rc < 0) return rc;
-  WubuB200ResNorm a = *p;
+  WubuB200ResNorm a = rc == 1 ? *p : as_ranges(*p);
   float* const out[kVectors] = {a.dweight, a.dbias, a.dpost_weight, a.dpost_bias, a.dgate};
   if (rc == 1) {  // no rows: the sums over them are zero
     for (int q = 0; q < kVectors; ++q) {
