@@ -12,6 +12,9 @@
 // write P back in two halves, from where the second product reads it as its A operand; a warp of its
 // own issues the stream's products.  While the warps of one stream work on their exponentials, the
 // tensor core runs the other stream's products.  K and V tiles arrive by TMA in rings and serve both.
+// Measured (B200): 16 heads on 4, 6000 tokens causal, 128 values: 160-170 us, 870-920 TFLOP/s of visible work
+// (floor 91 us at the measured product rate); 4 x 16 heads, 2048 x 64: 124 us; 16 x up to 499, 12 heads of 64:
+// 31 us (floor 4.9), of which a third is the filling and draining of items of four steps.
 // Up to 64 values a row, tensor memory has room for P beside S: the next scores are then issued as soon
 // as S has been read and the streams never wait for a product.  At 128 values P lies over S.
 #include <type_traits>
@@ -505,7 +508,8 @@ int launch_fwd(const AttnFwdMaps& maps, const AttnParams& p, cudaStream_t st) {
 
 }  // namespace
 
-// Few query rows and many keys: the keys of a row are split over CTAs, as many as fill the SMs once.
+// Few query rows and many keys: the keys of a row are split over CTAs, as many as fill the SMs once.  (One query
+// against 1500 keys, 12 heads: 10.5 + 7 us in 12 parts; unsplit, 12 tiles of about 1.6 us one after the other.)
 int attn_fwd_splits(const WubuB200Attn& a) {
   const long long ctas = (long long)((a.Tq + 2 * kTile - 1) / (2 * kTile)) * a.Hq * a.B;
   const int tiles = (a.Tk + kTile - 1) / kTile;

@@ -11,7 +11,9 @@
 // a range of one item's rows: the parameter vectors stay in registers, the next row is loaded before the
 // current one's sums are taken, and in the backward a thread meets the same columns in every row and
 // adds up the parameter gradients in registers; the blocks' partial sums are added in a fixed order by a
-// second kernel.
+// second kernel.  Measured (B200): 7984 x 768 bf16, rms / gate / rms: forward 13.4 us (49 MB: 56 % of the
+// measured copy rate), backward 30 + 6 us (74 MB); 6000 x 768 fp16 LayerNorm backward 18 + 5 us (46 MB).  The
+// backward's rows are bound by the latency of their four sums: 12 warps an SM hold all the registers.
 #include <type_traits>
 
 #include "ops.cuh"
