@@ -133,6 +133,20 @@ def test_long_sequences(D):
 
 
 @pytest.mark.parametrize("mask", list(MASKS))
+@pytest.mark.parametrize("shape", [(1, 2, 1, 1700, 1600, 64), (1, 2, 2, 1540, 1830, 128), (2, 6, 1, 300, 1570, 96),
+                                   (3, 2, 2, 1, 900, 64)], ids=str)
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+def test_items_in_parts(shape, mask, dtype):
+    """Few items of many steps, which are split and joined: of one role or both, whole, and with lengths that leave
+    parts without a step."""
+    q, k, v, dout = make(*shape, dtype, seed=sum(shape))
+    check(q, k, v, dout, **MASKS[mask])
+    B, Tq, Tk = shape[0], shape[3], shape[4]
+    lens = lambda T, first: torch.tensor([first, T // 2 + 1, 0][:B], dtype=torch.int32, device="cuda")  # noqa: E731
+    check(q, k, v, dout, q_lens=lens(Tq, min(Tq, 131)), k_lens=lens(Tk, 140), **MASKS[mask])
+
+
+@pytest.mark.parametrize("mask", list(MASKS))
 @pytest.mark.parametrize("T,D", [(300, 64), (130, 96), (70, 128)])
 @pytest.mark.parametrize("dtype", list(U), ids=str)
 def test_lengths_and_what_lies_beyond_them(mask, T, D, dtype):

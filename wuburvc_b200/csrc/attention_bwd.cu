@@ -19,8 +19,8 @@
 //                           dV(n) | dK(n) dP(n+1) S(n+2)             dS(n) | P(n+1)        up to 64
 //   queries' role:  tensor  dQ(n) dP(n+1) S(n+2)              warps  P(n+1) dS(n+1)
 //
-// Measured (B200): 16 heads on 4, 4001 tokens causal, 128 values: 264-279 us (floor 101 us for 5 products, 141
-// for the 7); 4 x 16 heads, 2048 x 64: 324 us; 16 x up to 499, 12 heads of 64: 72-76 us (floor 9.8).  What bounds
+// Measured (B200): 16 heads on 4, 4001 tokens causal, 128 values: 258 us alone (floor 101 us for 5 products, 141
+// for the 7); 4 x 16 heads, 2048 x 64: 319 us; 16 x up to 499, 12 heads of 64: 72-76 us (floor 9.8).  What bounds
 // it is the chain product - exponentials - product of a step: without any exponential it is 5 % faster.
 //
 // fp16 has few small numbers and a low ceiling, so its P is scaled by 2^14 (P <= 1) and its dS by the
@@ -629,16 +629,23 @@ long long tiles_of(int T) { return (T + kTile - 1) / kTile; }
 // Into how many parts the steps of a key tile's and of a query tile's item are split.  The grid is as long as its
 // longest item: where that (4 products a step in the keys' role, 3 in the other) is longer than an even
 // share of all the work, which happens with few heads or many that share a key head, it is cut to about
-// that share.  (4 x 4001 tokens causal, 16 query heads on 4: parts of 2.)  Causal order halves the work
-// but not the longest item.
+// that share.  Causal order halves the work but not the longest item.  Joining the parts costs what some 16
+// products do, and parts of fewer than six steps lose (12 heads on 1, 700 tokens, 64 values: 34 us with two steps
+// at least, 30 with six; at 400 tokens 31 and 27, four steps 25).  (us split / whole: 16 heads on 4,
+// 4001 tokens causal, 128 values, 2 parts: 258 / 309; 12 heads on 1, 1500 tokens, 64 values: 60 / 207; 12 heads,
+// 1500 causal, 64 values, the longest item 1.2 shares, so not split: 55 / 39; 2 heads of 96, 300 tokens, not split
+// either: 25 / 18.)
 void bwd_splits(const WubuB200Attn& a, int sms, int& kv, int& q) {
   const long long nq = tiles_of(a.Tq), nk = tiles_of(a.Tk), group = a.Hkv ? a.Hq / a.Hkv : 1;
   const long long kv_item = 4 * nq * group, q_item = 3 * nk;
   const long long share = (kv_item * nk * a.Hkv + q_item * nq * a.Hq) * a.B / (a.causal ? 2 : 1) / (sms > 0 ? sms : 1) + 1;
   auto parts = [&](long long item, long long steps) {
     long long s = (item + share - 1) / share;
-    if (s > (steps + 1) / 2) s = (steps + 1) / 2;  // two steps at least, for the prologue's sake
-    return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
+    if (s > steps / 6) s = steps / 6;
+    if (s > 16) s = 16;
+    if (s < 2) return 1;
+    const long long part = (item + s - 1) / s;
+    return item - (part > share ? part : share) > 16 ? (int)s : 1;
   };
   kv = parts(kv_item, nq * group);
   q = parts(q_item, nk);

@@ -12,9 +12,9 @@
 // write P back in two halves, from where the second product reads it as its A operand; a warp of its
 // own issues the stream's products.  While the warps of one stream work on their exponentials, the
 // tensor core runs the other stream's products.  K and V tiles arrive by TMA in rings and serve both.
-// Measured (B200): 16 heads on 4, 6000 tokens causal, 128 values: 160-170 us, 870-920 TFLOP/s of visible work
-// (floor 91 us at the measured product rate); 4 x 16 heads, 2048 x 64: 124 us; 16 x up to 499, 12 heads of 64:
-// 31 us (floor 4.9), of which a third is the filling and draining of items of four steps.
+// Measured (B200): 16 heads on 4, 6000 tokens causal, 128 values: 159 us, 930 TFLOP/s of visible work
+// (floor 91 us at the measured product rate); 4 x 16 heads, 2048 x 64: 117 us; 16 x up to 499, 12 heads of 64:
+// 31 us (floor 4.9): items of four steps, whose filling and draining nothing overlaps.
 // Up to 64 values a row, tensor memory has room for P beside S: the next scores are then issued as soon
 // as S has been read and the streams never wait for a product.  At 128 values P lies over S.
 #include <type_traits>
@@ -508,14 +508,18 @@ int launch_fwd(const AttnFwdMaps& maps, const AttnParams& p, cudaStream_t st) {
 
 }  // namespace
 
-// Few query rows and many keys: the keys of a row are split over CTAs, as many as fill the SMs once.  (One query
-// against 1500 keys, 12 heads: 10.5 + 7 us in 12 parts; unsplit, 12 tiles of about 1.6 us one after the other.)
+// Few query rows and many keys: the keys of a row are split over CTAs, as many as fill the SMs once, where that
+// takes more than three tiles off a CTA's chain: a tile is about 1.1 us of it, the join about 3 us.  (One query,
+// 64 values, us split / whole: 12 heads, 1500 keys 12.9 / 18.7, 600 keys 11.4 / 11.5, 400 keys 10.3 / 10.0, 200
+// keys 9.1 / 7.5; 72 heads, 1500 keys 17.1 / 19.3, 900 keys 14.8 / 15.8, 300 keys 12.8 / 9.7; 84 heads in two
+// parts, more than fill the SMs once, 1500 keys 27 / 19.4.)
 int attn_fwd_splits(const WubuB200Attn& a) {
   const long long ctas = (long long)((a.Tq + 2 * kTile - 1) / (2 * kTile)) * a.Hq * a.B;
   const int tiles = (a.Tk + kTile - 1) / kTile;
-  if (ctas == 0 || tiles < 2 || ctas > 74) return 1;
-  const long long s = 148 / ctas;
-  return (int)(s < tiles ? (s < kMaxSplits ? s : kMaxSplits) : tiles < kMaxSplits ? tiles : kMaxSplits);
+  if (ctas == 0 || ctas > 74) return 1;
+  const long long most = 148 / ctas < kMaxSplits ? 148 / ctas : kMaxSplits;
+  const int s = (int)(most < tiles ? most : tiles);
+  return s > 1 && tiles - (tiles + s - 1) / s > 3 ? s : 1;
 }
 long long attn_fwd_bytes(const WubuB200Attn& a) {
   const int s = attn_fwd_splits(a);

@@ -54,7 +54,6 @@ int ops_launch_after(void (*kernel)(Args...), dim3 grid, dim3 block, size_t smem
 inline bool ops_dtype_ok(int dtype) {
   return dtype == WUBU_B200_F32 || dtype == WUBU_B200_BF16 || dtype == WUBU_B200_F16;
 }
-inline size_t ops_dtype_bytes(int dtype) { return dtype == WUBU_B200_F32 ? 4 : 2; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 WB_DEV float to_float(float x) { return x; }
