@@ -12,8 +12,8 @@
 // write P back in two halves, from where the second product reads it as its A operand; a warp of its
 // own issues the stream's products.  While the warps of one stream work on their exponentials, the
 // tensor core runs the other stream's products.  K and V tiles arrive by TMA in rings and serve both.
-// Measured (B200): 16 heads on 4, 6000 tokens causal, 128 values: 159 us, 930 TFLOP/s of visible work
-// (floor 91 us at the measured product rate); 4 x 16 heads, 2048 x 64: 117 us; 16 x up to 499, 12 heads of 64:
+// Measured (B200): 16 heads on 4, 6000 tokens causal, 128 values: 159 us with its inputs in L2, 930
+// TFLOP/s of visible work, 170 without (floor 91 us at the measured product rate); 4 x 16 heads, 2048 x 64: 117 us; 16 x up to 499, 12 heads of 64:
 // 31 us (floor 4.9): items of four steps, whose filling and draining nothing overlaps.
 // Up to 64 values a row, tensor memory has room for P beside S: the next scores are then issued as soon
 // as S has been read and the streams never wait for a product.  At 128 values P lies over S.
