@@ -125,6 +125,27 @@ def test_many_heads(shape, dtype):
     check(*make(*shape, dtype, seed=7), causal=True)
 
 
+@pytest.mark.parametrize("shape", [(24, 8, 8, 300, 300, 128), (20, 8, 2, 260, 390, 96), (2, 16, 1, 1500, 1500, 128),
+                                   (24, 8, 8, 300, 300, 64)], ids=str)
+@pytest.mark.parametrize("mask", ["none", "causal"])
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+def test_many_padded_items(shape, mask, dtype):
+    """Several times more items than SMs, whole and in parts, many of them empty: a CTA meets an item without steps
+    between a keys' and a queries' item, whose second score tile at 128 values lies where dV is read from.  The same
+    bits every time."""
+    B, Hq, Hkv, Tq, Tk, D = shape
+    q, k, v, dout = make(*shape, dtype, seed=sum(shape))
+    lens = lambda T: torch.tensor([(T, T // 4, 3 * T // 5, 0, T // 2, 1)[b % 6] for b in range(B)], dtype=torch.int32, device="cuda")  # noqa: E731
+    opts = dict(q_lens=lens(Tq), k_lens=lens(Tk), **MASKS[mask])
+    check(q, k, v, dout, **opts)
+    out, lse = tf.attention_forward(q, k, v, **opts)
+    first = tf.attention_backward(dout, q, k, v, out, lse, **opts)
+    for _ in range(8):
+        again = tf.attention_backward(dout, q, k, v, out, lse, **opts)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+    tf.ops_sync()
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_long_sequences(D):
     """Many tiles an item: the rings go round, the running maximum and the sums span 20 tiles."""

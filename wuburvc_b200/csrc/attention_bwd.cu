@@ -282,10 +282,9 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
       const int ksteps = (a.D + 15) / 16;
       const uint64_t dr0 = desc_k(res0), dr1 = desc_k(res1);
       bool ok = true;
-      int n0 = 0, items = 0, p_count = 0;
-      int all = 0;  // items so far, those without steps too
+      int n0 = 0, items = 0, p_count = 0;  // steps, items (with steps) and halves of the keys' role so far
       Items take{bar, item_slots, 0};
-      for (BwdWork k; take.take(k, p); ++all) {
+      for (BwdWork k; take.take(k, p);) {
         take.done();
         if (k.steps == 0) continue;
         const bool kv = k.kv;
@@ -329,8 +328,10 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
         issue_s(0);
         issue_dp(0);
         if (two_s && k.steps > 1) {
-          // at 128 values the second S may still be the last item's dV
-          if (!kTwoS && ok && all) ok = bar_wait(&bar.acc_read, (all - 1) & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
+          // At 128 values the second S lies where the last item's dV may still be read.  Items without steps do not
+          // count on either side: the warps gave the last item's P and dS only after they had read the accumulators
+          // of the one before it, so the barrier is at most one phase behind and its parity tells which.
+          if (!kTwoS && ok && items > 1) ok = bar_wait(&bar.acc_read, (items - 2) & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
           tc_fence_after();
           issue_s(1);
         }
@@ -542,6 +543,7 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
           }
         }
       }
+      if (k.steps == 0) continue;
       tc_fence_before();  // the accumulators are read before the next item's products may be issued
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.acc_read);
