@@ -196,6 +196,46 @@ def test_peaked_scores(dtype):
     check(q, k, v, dout, causal=True)
 
 
+@pytest.mark.parametrize("what", ["nan", "inf"])
+@pytest.mark.parametrize("shape", [(1, 32, 32, 70, 200, 64), (1, 32, 32, 70, 200, 128), (1, 32, 32, 70, 200, 24),
+                                   (1, 32, 32, 2, 1500, 64), (1, 32, 32, 2, 1500, 128)], ids=str)
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+def test_live_keys_that_are_not_finite(shape, dtype, what):
+    """Head h has one key, at a place j = h (mod 32), whose score is NaN or +infinity for every query: whatever its
+    place in a tile, the rows that see it are NaN with a NaN lse, and the others have the bits that they have without it."""
+    _, H, _, Tq, Tk, D = shape
+    q, k, v, _ = make(*shape, dtype, seed=3)
+    q[..., 0] = 1
+    at = [Tk - 1 - (Tk - 1 - h) % 32 for h in range(H)]  # within the last 32 keys
+    for causal in (False, True):
+        clean = tf.attention_forward(q, k, v, causal=causal)
+        bad = k.clone()
+        for h, j in enumerate(at):
+            bad[0, j, h, 0] = math.nan if what == "nan" else math.inf
+        out, lse = tf.attention_forward(q, bad, v, causal=causal)
+        for h, j in enumerate(at):
+            sees = visible(Tq, Tk, causal, 0, Tq, Tk)[:, j]
+            assert out[0, sees, h].isnan().all() and lse[0, h, sees].isnan().all(), (h, j, causal)
+            assert torch.equal(out[0, ~sees, h], clean[0][0, ~sees, h]) and torch.equal(lse[0, h, ~sees], clean[1][0, h, ~sees])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+def test_live_keys_of_no_weight(dtype, D):
+    """Scores of -infinity: such keys have no weight, and a row that sees no others has out 0 and lse -inf."""
+    q, k, v, _ = make(1, 2, 2, 40, 150, D, dtype, seed=4)
+    q[..., 0] = 1
+    some, none = k.clone(), k.clone()
+    some[:, 100:, :, 0] = -math.inf
+    none[..., 0] = -math.inf
+    out, lse = tf.attention_forward(q, some, v)
+    lens = torch.tensor([100], dtype=torch.int32, device="cuda")
+    out2, lse2 = tf.attention_forward(q, k, v, k_lens=lens)
+    assert torch.equal(out, out2) and torch.equal(lse, lse2)
+    out, lse = tf.attention_forward(q, none, v)
+    assert (out == 0).all() and (lse == -math.inf).all()
+
+
 @pytest.mark.parametrize("size", [1e-3, 1.0, 300.0])
 @pytest.mark.parametrize("dtype", list(U), ids=str)
 def test_gradients_of_any_size(size, dtype):

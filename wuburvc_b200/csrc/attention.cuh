@@ -270,16 +270,18 @@ WB_DEV void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n
 template <int N>
 WB_DEV void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
+// The largest of three, NaN if one of them is.
 WB_DEV float max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
 // 2^x of two values on the FMA units, for x up to 120: x = n + f with n a whole number and |f| <= 1/2 (adding and
 // subtracting 1.5 * 2^23 rounds to n), 2^f by a polynomial of degree 4 whose largest relative error is
 // least (2.7e-6 in float32, far below the rounding of P; fitted by reweighted least squares), and n added
-// to the exponent.  Below -125 it returns about 2^-125, which stands for 0.
+// to the exponent.  Below -125, and for NaN, it returns about 2^-125, which stands for 0: a caller whose
+// values may be NaN looks for that elsewhere.
 WB_DEV uint64_t ex2_poly2(uint64_t x) {
   float a, b;
   each(x, a, b);

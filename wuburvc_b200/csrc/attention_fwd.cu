@@ -335,9 +335,11 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
         for (int k = 4; k < 124; k += 8)
 #pragma unroll
           for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[k + e], x[k + 4 + e]);
-        const float mt = max3(max3(mx[0], mx[1], x[124]), max3(mx[2], mx[3], x[125]), fmaxf(x[126], x[127]));
-        // move m when the maximum has outgrown it by 2^8 (or was not set)
-        const bool move = mt > m && (m == -INFINITY || (mt - m) * c > 8.f);
+        const float mt = max3(max3(mx[0], mx[1], x[124]), max3(mx[2], mx[3], x[125]), max3(x[126], x[127], x[127]));
+        // Move m when the maximum has outgrown it by 2^8 (or was not set), and where a score is NaN: the row's m is
+        // NaN from there on, and with it all that follows.  An infinite maximum makes it NaN too (infinity less
+        // itself is), as it does in the formula.
+        const bool move = !(mt <= m) && (m == -INFINITY || !((mt - m) * c <= 8.f));
         const bool any_move = __any_sync(0xffffffffu, move);
         // apart, S may be ahead of the product that last read P and added to O; over S it cannot be
         if (kApart && j > st0) ok = bar_wait(&pv_done[s], ph ^ 1u, p.err, ERR_WAIT_ACC, p.wait_ns);
@@ -345,7 +347,7 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
         if (!ok) continue;
         if (any_move) {
           const float f = !move ? 1.f : m == -INFINITY ? 0.f : ex2((m - mt) * c);
-          if (move) m = mt;
+          if (move) m = mt + (mt - mt);
           l *= f;
           if (j > st0) {
             tc_fence_after();
@@ -401,7 +403,8 @@ attn_fwd_tc_kernel(const __grid_constant__ AttnFwdMaps maps, const __grid_consta
       // the last product: its phase is that of the number of tiles before it
       if (st1 > st0 && ok) ok = bar_wait(&pv_done[s], ph ^ 1u, p.err, ERR_WAIT_ACC, p.wait_ns);
       tc_fence_after();
-      const bool live = l > 0.f && hi > lo && st1 > st0 && ok;
+      // (without a score above -infinity m is not set, and l holds what the polynomial's 2^-125 add up to)
+      const bool live = l > 0.f && m > -INFINITY && hi > lo && st1 > st0 && ok;
       const bool bad = hi > lo && st1 > st0 && !(l == l);  // a NaN among the scores stays visible
       const float inv = live ? 1.f / l : 0.f;
       const float lse = live ? m * a.scale + (logf(l) - kShift * 0.69314718055994531f) : bad ? l : -INFINITY;
