@@ -81,3 +81,13 @@ def test_training_lowers_the_loss():
         losses = encoder.train(steps=12, batch=4, frames=60, lr=1e-3, style=style, width=64, heads=2, hidden=128, layers=2,
                                report=lambda line: None)
         assert losses[-1] < 0.97 * losses[0] and all(x == x for x in losses)
+
+
+def test_second_derivatives_raise():
+    """Of the example's operators together: a gradient penalty is refused, not left out."""
+    model = encoder.Encoder(width=64, heads=2, hidden=128, layers=1, style="gated").cuda()
+    x = torch.randn(1, 20, 64, device="cuda").bfloat16().requires_grad_(True)
+    out = model(x, torch.tensor([20], dtype=torch.int32, device="cuda"), torch.randn(1, 256, device="cuda"))
+    g, = torch.autograd.grad(out.float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        (g.float().square().sum() + x.float().square().sum()).backward()

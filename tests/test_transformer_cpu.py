@@ -111,3 +111,78 @@ def test_binding_refuses_cpu_tensors():
                  lambda: tf.attention_forward(*(torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16),) * 3)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.fixture
+def stand_ins(monkeypatch):
+    """torch on the CPU in place of the native calls, as their outputs are to autograd: without a history.  Returns
+    the list of the calls' keyword arguments."""
+    calls = []
+
+    def called(name, f):
+        def g(*args, **kw):
+            calls.append((name, kw))
+            with torch.no_grad():
+                return f(*args, **kw)
+        monkeypatch.setattr(tf, name, g)
+
+    def scores(q, k):
+        return torch.einsum("bihd,bjhd->bhij", q, k) * q.shape[-1] ** -0.5
+
+    def attention_forward(q, k, v, **opts):
+        s = scores(q, k)
+        return torch.einsum("bhij,bjhd->bihd", torch.softmax(s, -1), v), torch.logsumexp(s, -1)
+
+    def attention_backward(dout, q, k, v, out, lse, **opts):
+        p = torch.exp(scores(q, k) - lse[..., None])
+        dp = torch.einsum("bihd,bjhd->bhij", dout, v)
+        ds = p * (dp - (p * dp).sum(-1, keepdim=True)) * q.shape[-1] ** -0.5
+        return (torch.einsum("bhij,bjhd->bihd", ds, k), torch.einsum("bhij,bihd->bjhd", ds, q),
+                torch.einsum("bhij,bihd->bjhd", p, dout))
+
+    def resnorm_forward(x, f, keep_sum=True, **kw):  # rms, without parameters
+        r = x + f
+        return r if keep_sum else None, r / torch.sqrt(r.square().mean(-1, keepdim=True) + 1e-5)
+
+    def resnorm_backward(dr, dh, x, f, **kw):
+        r = x + f
+        inv = 1 / torch.sqrt(r.square().mean(-1, keepdim=True) + 1e-5)
+        d = 0 if dr is None else dr
+        if dh is not None:
+            d = d + (dh - r * inv * (dh * r * inv).mean(-1, keepdim=True)) * inv
+        return dict(dx=d, df=d, **dict.fromkeys(("dweight", "dbias", "dpost_weight", "dpost_bias", "dgate")))
+
+    def act8_forward(x, act="gelu", slope=0.0, with_output=True):
+        return torch.nn.functional.gelu(x), tf.Kept8(x.clone(), x.new_ones(1), act, slope, x.dtype)
+
+    def act8_backward(dy, kept, recompute=False):
+        with torch.enable_grad():
+            x = kept.q.detach().requires_grad_(True)
+            y = torch.nn.functional.gelu(x)
+            dx, = torch.autograd.grad(y, x, dy)
+        return dx, y.detach()
+
+    for f in (attention_forward, attention_backward, resnorm_forward, resnorm_backward, act8_forward, act8_backward):
+        called(f.__name__, f)
+    return calls
+
+
+def autograd_forms():
+    """name -> (leaves, function of them) of each form, in float64"""
+    g = torch.Generator().manual_seed(0)
+    leaf = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64).requires_grad_(True)  # noqa: E731
+    return {
+        "attention": ([leaf(1, 5, 2, 8) for _ in range(3)], lambda q, k, v: tf.attention(q, k, v)),
+        "resnorm": ([leaf(2, 3, 8) for _ in range(2)], lambda x, f: sum(tf.resnorm(x, f, norm="rms"))),
+        "feed_forward": ([leaf(2, 3, 8), leaf(16, 8), leaf(16), leaf(8, 16), leaf(8)], tf.feed_forward),
+    }
+
+
+@pytest.mark.parametrize("form", ["attention", "resnorm", "feed_forward"])
+def test_first_derivatives_are_right_and_second_ones_raise(form, stand_ins):
+    leaves, f = autograd_forms()[form]
+    assert torch.autograd.gradcheck(f, leaves)
+    grads = torch.autograd.grad(f(*leaves).square().sum(), leaves, create_graph=True)
+    for g in grads:  # beside a term that can be differentiated
+        with pytest.raises(RuntimeError):
+            (g.square().sum() + leaves[0].square().sum()).backward(retain_graph=True)

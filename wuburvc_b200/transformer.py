@@ -6,7 +6,8 @@ besides their matrix products.
 * ``resnorm_forward`` / ``resnorm_backward``: the norms around a block, its gate and the residual scale;
 * ``attention_forward`` / ``attention_backward``: softmax attention, its gradient with the probabilities
   recomputed from the log-sum-exp;
-* ``attention``, ``resnorm``, ``feed_forward``: the same for torch's autograd.
+* ``attention``, ``resnorm``, ``feed_forward``: the same for torch's autograd, differentiable once (a second
+  derivative raises).
 
 Calls enqueue on the current torch stream of the tensors' device and do not synchronise; outputs are new
 tensors.  A call that cannot be made raises (``ValueError`` for its arguments, ``RuntimeError`` for a
@@ -21,6 +22,7 @@ import struct
 from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._lib import lib
 
@@ -410,6 +412,7 @@ class _Attention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         return (*attention_backward(dout, *ctx.saved_tensors, **ctx.opts), None)
 
@@ -429,6 +432,7 @@ class _ResNorm(torch.autograd.Function):
         return resnorm_forward(x, f, keep_sum=keep_sum, **vec, **opts)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dr, dh):
         x, f, *vec = ctx.saved_tensors
         if dr is None and dh is None:
@@ -453,6 +457,7 @@ class _FeedForward(torch.autograd.Function):
         return torch.nn.functional.linear(y, w2, b2)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         x, w1, w2, q, scale = ctx.saved_tensors
         act, slope, dtype, has_b1, has_b2 = ctx.kept
