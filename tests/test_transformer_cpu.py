@@ -186,3 +186,15 @@ def test_first_derivatives_are_right_and_second_ones_raise(form, stand_ins):
     for g in grads:  # beside a term that can be differentiated
         with pytest.raises(RuntimeError):
             (g.square().sum() + leaves[0].square().sum()).backward(retain_graph=True)
+
+
+@pytest.mark.parametrize("which", ["q_lens", "k_lens"])
+def test_lengths_changed_before_the_backward_are_noticed(which, stand_ins):
+    q, k, v = autograd_forms()["attention"][0]
+    lens = {n: torch.tensor([5], dtype=torch.int32) for n in ("q_lens", "k_lens")}
+    tf.attention(q, k, v, **lens).sum().backward()
+    assert all(kw["q_lens"] is not None and kw["k_lens"] is not None for _, kw in stand_ins)
+    out = tf.attention(q, k, v, **lens)
+    lens[which].fill_(3)  # the next batch's lengths in the same buffer
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()

@@ -405,21 +405,23 @@ def attention_backward(dout, q, k, v, out, lse, *, causal=False, window=0, scale
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, opts):
-        out, lse = attention_forward(q, k, v, **opts)
-        ctx.save_for_backward(q, k, v, out, lse)
+    def forward(ctx, q, k, v, q_lens, k_lens, opts):
+        out, lse = attention_forward(q, k, v, q_lens=q_lens, k_lens=k_lens, **opts)
+        # (the lengths among the saved tensors: changed in place before the backward, they raise there)
+        ctx.save_for_backward(q, k, v, out, lse, q_lens, k_lens)
         ctx.opts = opts
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        return (*attention_backward(dout, *ctx.saved_tensors, **ctx.opts), None)
+        *saved, q_lens, k_lens = ctx.saved_tensors
+        return (*attention_backward(dout, *saved, q_lens=q_lens, k_lens=k_lens, **ctx.opts), None, None, None)
 
 
-def attention(q, k, v, **opts):
+def attention(q, k, v, *, q_lens=None, k_lens=None, **opts):
     """``attention_forward``'s out, differentiable by torch's autograd."""
-    return _Attention.apply(q, k, v, opts)
+    return _Attention.apply(q, k, v, q_lens, k_lens, opts)
 
 
 class _ResNorm(torch.autograd.Function):
