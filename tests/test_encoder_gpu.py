@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from wuburvc_b200 import encoder
+from wuburvc_b200 import transformer as tf
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +92,33 @@ def test_second_derivatives_raise():
     g, = torch.autograd.grad(out.float().square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         (g.float().square().sum() + x.float().square().sum()).backward()
+
+
+def test_autocast():
+    """float32 leaves under autocast: the bits that the same calls give on leaves cast by hand, and gradients that are
+    those rounded to no more than the leaves' type."""
+    rnd = torch.Generator(device="cuda").manual_seed(5)
+    leaf = lambda *s: torch.randn(*s, generator=rnd, device="cuda").requires_grad_(True)  # noqa: E731
+    qkv = [leaf(2, 33, 4, 64) for _ in range(3)]
+    ffn = [leaf(2, 33, 64), leaf(128, 64), leaf(128), leaf(64, 128), leaf(64)]
+    for leaves, f in ((qkv, tf.attention), (ffn, tf.feed_forward)):
+        hand = [t.detach().bfloat16().requires_grad_(True) for t in leaves]
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            out = f(*leaves)
+        out.float().square().sum().backward()
+        want = f(*hand)
+        want.float().square().sum().backward()
+        assert torch.equal(out, want)
+        for t, h in zip(leaves, hand):
+            assert t.grad.dtype == torch.float32 and torch.equal(t.grad, h.grad.float())
+    x, f = leaf(2, 33, 64), leaf(2, 33, 64).detach().bfloat16().requires_grad_(True)
+    with torch.autocast("cuda", dtype=torch.bfloat16):  # a float32 sum and a block's 16-bit result
+        r, h = tf.resnorm(x, f)
+    (r.square().sum() + (h * x.detach()).sum()).backward()
+    wide = [t.detach().float().requires_grad_(True) for t in (x, f)]
+    r2, h2 = tf.resnorm(*wide)
+    (r2.square().sum() + (h2 * x.detach()).sum()).backward()
+    assert torch.equal(r, r2) and torch.equal(h, h2)
+    assert torch.equal(x.grad, wide[0].grad) and torch.equal(f.grad, wide[1].grad.bfloat16())
+    with pytest.raises(ValueError):
+        tf.resnorm(x, f)  # outside a region types are the caller's

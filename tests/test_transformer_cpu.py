@@ -198,3 +198,25 @@ def test_lengths_changed_before_the_backward_are_noticed(which, stand_ins):
     lens[which].fill_(3)  # the next batch's lengths in the same buffer
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.sum().backward()
+
+
+@pytest.mark.parametrize("inside", [False, True])
+@pytest.mark.parametrize("form", ["attention", "resnorm", "feed_forward"])
+def test_autocast(form, inside, stand_ins):
+    """float32 leaves under autocast: what the native calls see is in one type, the gradients come back in the leaves'
+    type and near the float64 ones (bf16 roundings of a few terms: 2^-9 each, 2 % holds ten in a row), whether
+    the backward runs inside the region or outside."""
+    leaves, f = autograd_forms()[form]
+    want = torch.autograd.grad(f(*leaves).square().sum(), leaves)
+    low = [t.detach().float().requires_grad_(True) for t in leaves]
+    if form == "resnorm":  # a float32 sum and a block's 16-bit result
+        low[1] = low[1].detach().bfloat16().requires_grad_(True)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        out = f(*low)
+        assert out.dtype == (torch.float32 if form == "resnorm" else torch.bfloat16)
+        if inside:
+            out.float().square().sum().backward()
+    if not inside:
+        out.float().square().sum().backward()
+    for t, w in zip(low, want):
+        assert t.grad.dtype == t.dtype and (t.grad.double() - w).norm() <= 0.02 * w.norm()

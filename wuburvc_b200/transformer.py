@@ -403,6 +403,16 @@ def attention_backward(dout, q, k, v, out, lse, *, causal=False, window=0, scale
     return dq, dk, dv
 
 
+def _autocast(*ts, to=None):
+    """Under torch.autocast, ``ts`` (None left out) in the type ``to``, by default autocast's, cast where autograd sees
+    it; else as they are.  float64 is left alone, as torch leaves it."""
+    kind = ts[0].device.type
+    if not torch.is_autocast_enabled(kind):
+        return ts
+    to = to or torch.get_autocast_dtype(kind)
+    return tuple(t if t is None or t.dtype not in _DTYPES else t.to(to) for t in ts)
+
+
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_lens, k_lens, opts):
@@ -420,8 +430,8 @@ class _Attention(torch.autograd.Function):
 
 
 def attention(q, k, v, *, q_lens=None, k_lens=None, **opts):
-    """``attention_forward``'s out, differentiable by torch's autograd."""
-    return _Attention.apply(q, k, v, q_lens, k_lens, opts)
+    """``attention_forward``'s out, differentiable by torch's autograd.  Under autocast in its type."""
+    return _Attention.apply(*_autocast(q, k, v), q_lens, k_lens, opts)
 
 
 class _ResNorm(torch.autograd.Function):
@@ -446,7 +456,9 @@ class _ResNorm(torch.autograd.Function):
 
 
 def resnorm(x, f, *, weight=None, bias=None, post_weight=None, post_bias=None, gate=None, keep_sum=True, **opts):
-    """``resnorm_forward``'s (r, h), differentiable by torch's autograd.  Only x and f are kept for the backward."""
+    """``resnorm_forward``'s (r, h), differentiable by torch's autograd.  Only x and f are kept for the backward.  Under
+    autocast x and f may differ in type: the wider one counts."""
+    x, f = _autocast(x, f, to=torch.promote_types(x.dtype, f.dtype))
     return _ResNorm.apply(x, f, weight, bias, post_weight, post_bias, gate, opts, keep_sum)
 
 
@@ -463,15 +475,16 @@ class _FeedForward(torch.autograd.Function):
     def backward(ctx, dout):
         x, w1, w2, q, scale = ctx.saved_tensors
         act, slope, dtype, has_b1, has_b2 = ctx.kept
-        du, y = act8_backward(dout @ w2, Kept8(q, scale, act, slope, dtype), recompute=True)
-        rows = lambda t: t.reshape(-1, t.shape[-1])  # noqa: E731
-        dw1, dw2 = rows(du).T @ rows(x), rows(dout).T @ rows(y)
-        db1 = rows(du).sum(0) if has_b1 else None
-        db2 = rows(dout).sum(0) if has_b2 else None
-        return du @ w1, dw1, db1, dw2, db2, None, None
+        with torch.autocast(x.device.type, enabled=False):  # the saved tensors are in the forward's type
+            du, y = act8_backward(dout @ w2, Kept8(q, scale, act, slope, dtype), recompute=True)
+            rows = lambda t: t.reshape(-1, t.shape[-1])  # noqa: E731
+            dw1, dw2 = rows(du).T @ rows(x), rows(dout).T @ rows(y)
+            db1 = rows(du).sum(0) if has_b1 else None
+            db2 = rows(dout).sum(0) if has_b2 else None
+            return du @ w1, dw1, db1, dw2, db2, None, None
 
 
 def feed_forward(x, w1, b1, w2, b2, act="gelu", slope=0.0):
     """act(x w1^T + b1) w2^T + b2, differentiable.  Of its hidden layer the backward keeps the 8-bit form alone: the
-    activation's derivative and the input of w2's gradient are both formed from it."""
-    return _FeedForward.apply(x, w1, b1, w2, b2, act, slope)
+    activation's derivative and the input of w2's gradient are both formed from it.  Under autocast in its type."""
+    return _FeedForward.apply(*_autocast(x, w1, b1, w2, b2), act, slope)
