@@ -153,6 +153,18 @@ def test_zero_rows_and_nan_stay_in_their_row():
     assert (e["dweight"] == 0).all() and (e["dgate"] == 0).all() and e["dgate"].shape == (2, 64)
 
 
+@pytest.mark.parametrize("C", [96, 97, 4000])
+def test_each_gradient_alone(C):
+    """`need` leaves outputs out; what is left has the same bits."""
+    t, dr, dh = make((3, 50, C), torch.bfloat16, "layer", "layer", "item")
+    kw = dict(norm="layer", post="layer", **{n: t[n] for n in NAMES})
+    want = tf.resnorm_backward(dr, dh, t["x"], t["f"], **kw)
+    assert all(v is not None for v in want.values())
+    for n, v in want.items():
+        got = tf.resnorm_backward(dr, dh, t["x"], t["f"], need=[n], **kw)
+        assert torch.equal(got.pop(n), v) and all(u is None for u in got.values())
+
+
 def test_deterministic():
     t, dr, dh = make((4, 500, 768), torch.bfloat16, "rms", "rms", "item")
     kw = dict(norm="rms", post="rms", **{n: t[n] for n in NAMES})

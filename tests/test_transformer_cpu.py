@@ -116,12 +116,12 @@ def test_binding_refuses_cpu_tensors():
 @pytest.fixture
 def stand_ins(monkeypatch):
     """torch on the CPU in place of the native calls, as their outputs are to autograd: without a history.  Returns
-    the list of the calls' keyword arguments."""
+    the list of the calls: (name, arguments, keyword arguments)."""
     calls = []
 
     def called(name, f):
         def g(*args, **kw):
-            calls.append((name, kw))
+            calls.append((name, args, kw))
             with torch.no_grad():
                 return f(*args, **kw)
         monkeypatch.setattr(tf, name, g)
@@ -159,7 +159,7 @@ def stand_ins(monkeypatch):
         with torch.enable_grad():
             x = kept.q.detach().requires_grad_(True)
             y = torch.nn.functional.gelu(x)
-            dx, = torch.autograd.grad(y, x, dy)
+            dx = None if dy is None else torch.autograd.grad(y, x, dy)[0]
         return dx, y.detach()
 
     for f in (attention_forward, attention_backward, resnorm_forward, resnorm_backward, act8_forward, act8_backward):
@@ -193,7 +193,7 @@ def test_lengths_changed_before_the_backward_are_noticed(which, stand_ins):
     q, k, v = autograd_forms()["attention"][0]
     lens = {n: torch.tensor([5], dtype=torch.int32) for n in ("q_lens", "k_lens")}
     tf.attention(q, k, v, **lens).sum().backward()
-    assert all(kw["q_lens"] is not None and kw["k_lens"] is not None for _, kw in stand_ins)
+    assert all(kw["q_lens"] is not None and kw["k_lens"] is not None for _, _, kw in stand_ins)
     out = tf.attention(q, k, v, **lens)
     lens[which].fill_(3)  # the next batch's lengths in the same buffer
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
@@ -220,3 +220,33 @@ def test_autocast(form, inside, stand_ins):
         out.float().square().sum().backward()
     for t, w in zip(low, want):
         assert t.grad.dtype == t.dtype and (t.grad.double() - w).norm() <= 0.02 * w.norm()
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_frozen_operands_of_feed_forward(which, stand_ins):
+    """One operand trained: its gradient is that of training all, and the native call is asked for no more than
+    it takes."""
+    leaves, f = autograd_forms()["feed_forward"]
+    want = torch.autograd.grad(f(*leaves).square().sum(), leaves)[which]
+    f(*(t if n == which else t.detach() for n, t in enumerate(leaves))).square().sum().backward()
+    assert torch.allclose(leaves[which].grad, want, rtol=1e-12, atol=0)
+    assert all(t.grad is None for n, t in enumerate(leaves) if n != which)
+    asked = [(a[0] is not None, kw["recompute"]) for name, a, kw in stand_ins if name == "act8_backward"][1:]
+    assert asked == {0: [(True, False)], 1: [(True, False)], 2: [(True, False)], 3: [(False, True)], 4: []}[which]
+
+
+@pytest.mark.parametrize("which", range(7))
+def test_frozen_operands_of_resnorm(which, monkeypatch):
+    asked = []
+
+    def backward(dr, dh, x, f, need=None, **kw):
+        asked.append(need)
+        return {n: torch.zeros(8) if n in need else None for n in
+                ("dx", "df", "dweight", "dbias", "dpost_weight", "dpost_bias", "dgate")}
+
+    monkeypatch.setattr(tf, "resnorm_forward", lambda x, f, **kw: (x + f, x - f))
+    monkeypatch.setattr(tf, "resnorm_backward", backward)
+    names = ("x", "f", "weight", "bias", "post_weight", "post_bias", "gate")
+    t = {n: torch.ones(8).requires_grad_(m == which) for m, n in enumerate(names)}
+    tf.resnorm(t.pop("x"), t.pop("f"), norm="layer", post="layer", **t)[1].sum().backward()
+    assert asked == [["d" + names[which]]]

@@ -257,10 +257,11 @@ def resnorm_forward(x, f, *, norm="layer", weight=None, bias=None, post=None, po
 
 
 def resnorm_backward(dr, dh, x, f, *, norm="layer", weight=None, bias=None, post=None, post_weight=None,
-                     post_bias=None, gate=None, res_scale=1.0, eps=1e-5):
+                     post_bias=None, gate=None, res_scale=1.0, eps=1e-5, need=None):
     """Gradients of ``resnorm_forward`` for the gradients ``dr`` of r and ``dh`` of h (either may be
     None): a dict of dx, df, dgate, dweight, dbias, dpost_weight, dpost_bias, None for what the
-    operator was not given.  The vectors' gradients are float32 sums over the rows."""
+    operator was not given, or what ``need`` (names of the dict; None: all) leaves out.  The vectors' gradients are
+    float32 sums over the rows."""
     what = "resnorm_backward"
     d = _dtype(x, what)
     dev, items, rows, C, vec, kind, gate = _resnorm_operands(what, x, f, norm, weight, bias, post, post_weight,
@@ -280,22 +281,21 @@ def resnorm_backward(dr, dh, x, f, *, norm="layer", weight=None, bias=None, post
     dr, dh = grads
     x, xs = _rows(x)
     f, fs = _rows(f)
-    dx = _empty(x)
-    df = _empty(x)
-    dweight, dbias, dpost_weight, dpost_bias, dgate = (v if v is None else torch.empty_like(v) for v in (*vec, gate))
+    out = {}
+    for n, v in zip(("dx", "df", "dweight", "dbias", "dpost_weight", "dpost_bias", "dgate"), (x, x, *vec, gate)):
+        out[n] = None if v is None or (need is not None and n not in need) else _empty(v)
 
     def pack(ws, n):
         return _RESNORM.pack(d, _NORMS[norm], _NORMS[post], kind, items, rows, C, res_scale, eps, 0, x.data_ptr(), xs,
                              f.data_ptr(), fs, *map(_ptr, vec), _ptr(gate), 0, 0, _ptr(dr), strides[0], _ptr(dh),
-                             strides[1], dx.data_ptr(), df.data_ptr(), _ptr(dgate), _ptr(dpost_weight),
-                             _ptr(dpost_bias), _ptr(dweight), _ptr(dbias), ws, n)
+                             strides[1], *(_ptr(out[m]) for m in ("dx", "df", "dgate", "dpost_weight", "dpost_bias", "dweight",
+                                                                  "dbias")), ws, n)
 
     h = L()
     n = _check(h.wubu_b200_resnorm_workspace(pack(0, 0)), what)
     ws = x.new_empty(n, dtype=torch.uint8)
     _call(what, h.wubu_b200_resnorm_backward, dev, pack(ws.data_ptr(), n))
-    return {"dx": dx, "df": df, "dgate": dgate, "dweight": dweight, "dbias": dbias, "dpost_weight": dpost_weight,
-            "dpost_bias": dpost_bias}
+    return out
 
 
 # ---- attention --------------------------------------------------------------------------------------
@@ -450,8 +450,9 @@ class _ResNorm(torch.autograd.Function):
         if dr is None and dh is None:
             return (None,) * 9
         names = ("weight", "bias", "post_weight", "post_bias", "gate")
-        g = resnorm_backward(dr, dh, x, f, **dict(zip(names, vec)), **ctx.opts)
-        cast = [None if v is None else g["d" + n].to(v.dtype) for n, v in zip(names, vec)]
+        need = [n for n, wanted in zip(("dx", "df", *("d" + n for n in names)), ctx.needs_input_grad) if wanted]
+        g = resnorm_backward(dr, dh, x, f, **dict(zip(names, vec)), **ctx.opts, need=need)
+        cast = [g["d" + n] if g["d" + n] is None else g["d" + n].to(v.dtype) for n, v in zip(names, vec)]
         return (g["dx"], g["df"], *cast, None, None)
 
 
@@ -467,21 +468,32 @@ class _FeedForward(torch.autograd.Function):
     def forward(ctx, x, w1, b1, w2, b2, act, slope):
         y, kept = act8_forward(torch.nn.functional.linear(x, w1, b1), act, slope=slope)
         ctx.save_for_backward(x, w1, w2, kept.q, kept.scale)
-        ctx.kept = (kept.act, kept.slope, kept.dtype, b1 is not None, b2 is not None)
+        ctx.kept = (kept.act, kept.slope, kept.dtype)
         return torch.nn.functional.linear(y, w2, b2)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         x, w1, w2, q, scale = ctx.saved_tensors
-        act, slope, dtype, has_b1, has_b2 = ctx.kept
+        act, slope, dtype = ctx.kept
+        need_x, need_w1, need_b1, need_w2, need_b2 = ctx.needs_input_grad[:5]
+        rows = lambda t: t.reshape(-1, t.shape[-1])  # noqa: E731
+        dx = dw1 = db1 = dw2 = db2 = None
         with torch.autocast(x.device.type, enabled=False):  # the saved tensors are in the forward's type
-            du, y = act8_backward(dout @ w2, Kept8(q, scale, act, slope, dtype), recompute=True)
-            rows = lambda t: t.reshape(-1, t.shape[-1])  # noqa: E731
-            dw1, dw2 = rows(du).T @ rows(x), rows(dout).T @ rows(y)
-            db1 = rows(du).sum(0) if has_b1 else None
-            db2 = rows(dout).sum(0) if has_b2 else None
-            return du @ w1, dw1, db1, dw2, db2, None, None
+            inner = need_x or need_w1 or need_b1
+            if inner or need_w2:
+                du, y = act8_backward(dout @ w2 if inner else None, Kept8(q, scale, act, slope, dtype), recompute=need_w2)
+            if need_x:
+                dx = du @ w1
+            if need_w1:
+                dw1 = rows(du).T @ rows(x)
+            if need_b1:
+                db1 = rows(du).sum(0)
+            if need_w2:
+                dw2 = rows(dout).T @ rows(y)
+            if need_b2:
+                db2 = rows(dout).sum(0)
+        return dx, dw1, db1, dw2, db2, None, None
 
 
 def feed_forward(x, w1, b1, w2, b2, act="gelu", slope=0.0):
