@@ -340,7 +340,7 @@ int wubu_b200_ops_sync(void* stream);
  *             values of a row (the last block of a row may be shorter): scale = max|x| / 127,
  *             q = round-to-even(x * (127 / max|x|)).  A block whose max|x| is below 2^-100 is kept
  *             as zeros; a block that holds an infinity or a NaN gets scale NaN, and all of it is
- *             restored as NaN.
+ *             restored as NaN, with derivatives that are NaN (but for the identity's, which is 1).
  *   backward: with x' = q * scale, dx = dy * act'(x') and, where asked for, y' = act(x') (what the
  *             next layer's weight gradient reads, so that y need not be kept either).
  * act: WUBU_B200_ACT_*; slope: of the leaky ReLU (0 = ReLU), whose derivative at 0 is the slope.  A value within

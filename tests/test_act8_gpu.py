@@ -108,6 +108,20 @@ def test_zeros_tiny_values_infinities_and_nan(C):
     assert back[2, 128:].isfinite().all() and back[3, :256].isfinite().all()
 
 
+@pytest.mark.parametrize("C", [384, 381])
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+@pytest.mark.parametrize("act,slope", [("gelu", 0.0), ("silu", 0.0), ("lrelu", 0.0), ("lrelu", 0.1), ("lrelu_sign", 0.0)])
+def test_a_block_that_is_not_finite_has_no_finite_gradient(act, slope, dtype, C):
+    """An overflow shows in the gradient under every activation, and in its own block alone."""
+    x, dy = torch.randn(4, C).to(dtype), torch.randn(4, C).to(dtype)
+    x[2, 5] = math.inf
+    x[3, 300] = math.nan
+    _, kept = tf.act8_forward(x.cuda(), act, slope=slope)
+    for t in tf.act8_backward(dy.cuda(), kept, recompute=True):
+        assert t[2, :128].isnan().all() and t[3, 256:].isnan().all()
+        assert t[:2].isfinite().all() and t[2, 128:].isfinite().all() and t[3, :256].isfinite().all()
+
+
 def test_gradient_against_differences():
     """dx dy-weighted against central differences of the forward at the restored point (float32): the
     third derivative of gelu is below 2, so a step of 1e-2 is off by 4e-5, rounding by 1e-7 / 1e-2."""

@@ -87,6 +87,9 @@ WB_DEV uint64_t act_value2(uint64_t x, float slope) {
   if (ACT == WUBU_B200_ACT_SILU) return mul2(x, rcp2(add2(both(1.f), ex22(mul2(x, both(-1.4426950408889634f))))));
   return x;
 }
+// The slope that the backward of a block with this scale takes: NaN where the block is kept as NaN, so that the
+// leaky ReLU's derivative, which looks at x' > 0 alone, is NaN there as the others' are.
+WB_DEV float slope_of(float slope, float scale) { return scale == scale ? slope : scale; }
 // act(x) and act'(x)
 template <int ACT>
 WB_DEV void act_both2(uint64_t x, float slope, uint64_t& y, uint64_t& d) {
@@ -214,7 +217,7 @@ __global__ void __launch_bounds__(kThreads) act8_backward_kernel(const Act8 a) {
   if (blk >= a.blocks) return;
   const long long row = a.nblk == 1 ? blk : blk / a.nblk;
   const int c0 = (int)(blk - row * a.nblk) * kBlock + t * 8;
-  const float scale = __ldg(a.scale + blk);
+  const float scale = __ldg(a.scale + blk), slope = slope_of(a.slope, scale);
   const long long at = row * a.cols + c0;
   uint2 q[2];
   float g[2][8];
@@ -234,7 +237,7 @@ __global__ void __launch_bounds__(kThreads) act8_backward_kernel(const Act8 a) {
       const uint32_t w = k < 4 ? lo : hi;
       const uint64_t x = mul2(two(dequantise(w, k & 3), dequantise(w, (k & 3) + 1)), both(scale));
       uint64_t yy, d;
-      act_both2<ACT>(x, a.slope, yy, d);
+      act_both2<ACT>(x, slope, yy, d);
       each(yy, y[k], y[k + 1]);
       each(mul2(two(g[i][k], g[i][k + 1]), d), g[i][k], g[i][k + 1]);
     }
@@ -288,7 +291,7 @@ __global__ void __launch_bounds__(kThreads) act8_backward_any_kernel(const Act8 
   if (blk >= a.blocks) return;
   const long long row = blk / a.nblk;
   const int c0 = (int)(blk - row * a.nblk) * kBlock + lane;
-  const float scale = a.scale[blk];
+  const float scale = a.scale[blk], slope = slope_of(a.slope, scale);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int c = c0 + 32 * i;
@@ -296,7 +299,7 @@ __global__ void __launch_bounds__(kThreads) act8_backward_any_kernel(const Act8 
     const long long at = row * a.cols + c;
     uint64_t yy, dd;
     float y, d, unused;
-    act_both2<ACT>(two((float)a.q[at] * scale, 0.f), a.slope, yy, dd);
+    act_both2<ACT>(two((float)a.q[at] * scale, 0.f), slope, yy, dd);
     each(yy, y, unused);
     each(dd, d, unused);
     if (a.out)
