@@ -346,7 +346,7 @@ int wubu_b200_ops_sync(void* stream);
  * act: WUBU_B200_ACT_*; slope: of the leaky ReLU (0 = ReLU), whose derivative at 0 is the slope.  A value within
  * half a step above 0 is kept as 0, so its derivative under ACT_LRELU is the slope's (about 0.5 % of
  * normally distributed values: a tenth of the gradient's norm); ACT_LRELU_SIGN keeps it as one step and
- * every derivative is that of x.
+ * every derivative is that of x (positive values of a block below 2^-100 as a step of 2^-100 / 127).
  * x, dy: `rows` rows of `cols` values, row strides in elements; y, q, dx, y_again: contiguous rows;
  * scale: [rows][ceil(cols / 128)].  y may be NULL (checkpoint only); dy and dx may both be NULL
  * (y_again only: with WUBU_B200_ACT_IDENTITY this restores x'). */

@@ -150,6 +150,22 @@ def test_lrelu_sign_keeps_every_derivative(C, dtype):
     assert ((again.float() - y.float()).abs() <= 1.01 * step + U[dtype] * y.float().abs()).all()
 
 
+@pytest.mark.parametrize("C", [256, 250])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_lrelu_sign_of_tiny_blocks(C, dtype):
+    """Blocks below 2^-100, with zeros among them, keep their derivatives too; x' is off by 2^-100 at most, and a block
+    of zeros is restored as zeros."""
+    x = (torch.randn(6, C) * 2.0 ** -110).to(dtype).cuda()
+    x[:, ::5] = 0
+    x[1, :128] = 0
+    x[2, 128:] *= 2.0 ** -12  # float32: subnormal
+    dy = torch.randn(6, C).to(dtype).cuda()
+    _, kept = tf.act8_forward(x, "lrelu_sign", slope=0.25)
+    dx, again = tf.act8_backward(dy, kept, recompute=True)
+    assert torch.equal(dx, torch.where(x > 0, dy, (dy.float() * 0.25).to(dtype)))
+    assert (again.double() - x.double()).abs().max() <= 2.0 ** -100 and (again[1, :128] == 0).all()
+
+
 def test_empty():
     for shape in ((0, 64), (3, 0)):
         x = torch.empty(shape, device="cuda", dtype=torch.bfloat16)

@@ -18,7 +18,7 @@ namespace {
 
 constexpr int kBlock = 128;        // values that share a scale
 constexpr int kThreads = 256;
-constexpr float kTiny = 0x1p-100f;  // below this a block is kept as zeros (127 / max|x| must not overflow)
+constexpr float kTiny = 0x1p-100f;  // below this a block is kept as zeros (127 / max|x| must not overflow), but see block_scale
 
 struct Act8 {
   float slope;
@@ -140,10 +140,12 @@ WB_DEV uint32_t abs_bits8(const uint4* r, f16) {
   return __float_as_uint(__half2float(__ushort_as_half((unsigned short)abs_halves(r))));
 }
 
+// ACT_LRELU_SIGN keeps the positive values of a tiny block too, as one step of kTiny / 127.
+template <int ACT>
 WB_DEV void block_scale(uint32_t top, float& inv, float& scale) {
   const float m = __uint_as_float(top);
   inv = m < kTiny ? 0.f : __fdiv_rn(127.f, m);
-  scale = m < kTiny ? 0.f : __fdiv_rn(m, 127.f);
+  scale = m < kTiny ? (ACT == WUBU_B200_ACT_LRELU_SIGN && m > 0.f ? kTiny / 127.f : 0.f) : __fdiv_rn(m, 127.f);
   if (top >= 0x7F800000u) {  // an infinity or a NaN in the block
     inv = 0.f;
     scale = __uint_as_float(0x7FC00000u);
@@ -186,7 +188,7 @@ __global__ void __launch_bounds__(kThreads) act8_forward_kernel(const Act8 a) {
   for (int m = 1; m < 8; m <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, m));
   if (!on) return;
   float inv, scale;
-  block_scale(top, inv, scale);
+  block_scale<ACT>(top, inv, scale);
   if (t == 0) a.scale[blk] = scale;
   const bool bad = top >= 0x7F800000u;  // q = 0 there (x * 0 may be NaN)
 #pragma unroll
@@ -264,7 +266,7 @@ __global__ void __launch_bounds__(kThreads) act8_forward_any_kernel(const Act8 a
   }
   top = __reduce_max_sync(0xffffffffu, top);
   float inv, scale;
-  block_scale(top, inv, scale);
+  block_scale<ACT>(top, inv, scale);
   if (lane == 0) a.scale[blk] = scale;
   const bool bad = top >= 0x7F800000u;
   uint32_t q[4];
