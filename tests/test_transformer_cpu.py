@@ -250,3 +250,27 @@ def test_frozen_operands_of_resnorm(which, monkeypatch):
     t = {n: torch.ones(8).requires_grad_(m == which) for m, n in enumerate(names)}
     tf.resnorm(t.pop("x"), t.pop("f"), norm="layer", post="layer", **t)[1].sum().backward()
     assert asked == [["d" + names[which]]]
+
+
+def test_workspaces_are_asked_for_on_the_tensors_device(monkeypatch):
+    """Two devices whose workspaces differ: each is asked for with its own device current, whichever was first."""
+    import contextlib
+    current = [0]
+
+    @contextlib.contextmanager
+    def device(dev):
+        before, current[0] = current[0], dev
+        yield
+        current[0] = before
+
+    class Library:
+        def wubu_b200_attn_workspace(self, args, backward):
+            return 1000 * (1 + current[0]) + backward
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(tf, "L", Library)
+    tf._workspace.cache_clear()
+    head = (1, 2, 4, 2, 10, 12, 64, 0, 0, 0.0)
+    assert [tf._workspace(dev, head, b) for b in (0, 1) for dev in (1, 0, 1)] == [2000, 1000, 2000, 2001, 1001, 2001]
+    tf._workspace.cache_clear()

@@ -1,5 +1,4 @@
 // attention.cu — softmax attention and its gradient: entry points and argument checks.
-#include <atomic>
 #include <cmath>
 
 #include "attention.cuh"
@@ -13,15 +12,6 @@ bool attn_map(CUtensorMap* m, const WubuB200View& v, int B, int T, int H, int D)
   const uint64_t strides[3] = {v.token ? (uint64_t)v.token * 2 : 16, v.head ? (uint64_t)v.head * 2 : 16,
                                v.batch ? (uint64_t)v.batch * 2 : 16};
   return make_map_16bit_4d(m, v.data, dims, strides, 64, kTile);
-}
-
-int attn_sms() {
-  static std::atomic<int> sms[64];
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-  n = sms[dev].load();
-  if (!n && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) sms[dev].store(n);
-  return n;
 }
 
 namespace {

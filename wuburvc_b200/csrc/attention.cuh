@@ -66,7 +66,6 @@ struct AttnRounds {
     next = round * (int)gridDim.x + ((round & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
   }
 };
-int attn_sms();  // SMs of the current device
 
 int attn_forward(const AttnParams& p, cudaStream_t st);
 long long attn_fwd_bytes(const WubuB200Attn& a);  // the forward's workspace

@@ -692,7 +692,7 @@ int launch_bwd(const AttnBwdMaps& maps, const AttnParams& p, int sms, cudaStream
 // The workspace: delta, lse2, counter and norm bits (to a multiple of 16 bytes), then the parts of dk, dv and dq.
 long long bwd_layout(const WubuB200Attn& a, AttnParams* p) {
   int kv = 1, q = 1;
-  bwd_splits(a, attn_sms(), kv, q);
+  bwd_splits(a, ops_sms(), kv, q);
   const long long rows = (long long)a.B * a.Hq * tiles_of(a.Tq) * kTile, bits = (1 + 2ll * a.B * a.Hkv + 3) / 4 * 4;
   const long long dkv = kv > 1 ? (long long)kv * a.B * a.Hkv * a.Tk * a.D : 0;
   const long long dq = q > 1 ? (long long)q * a.B * a.Hq * a.Tq * a.D : 0;
@@ -719,7 +719,7 @@ int attn_backward(const AttnParams& in, cudaStream_t st) {
   AttnParams p = in;
   const WubuB200Attn& a = p.a;
   bwd_layout(a, &p);
-  const int sms = attn_sms();
+  const int sms = ops_sms();
   if (!sms) return WUBU_B200_ERR_CUDA;
   AttnBwdMaps maps{};
   if (a.Tq && (!attn_map(&maps.q, a.q, a.B, a.Tq, a.Hq, a.D) || !attn_map(&maps.dout, a.dout, a.B, a.Tq, a.Hq, a.D)))

@@ -493,7 +493,7 @@ int launch_fwd(const AttnFwdMaps& maps, const AttnParams& p, cudaStream_t st) {
   static std::atomic<uint64_t> devices{0};
   if (!ops_smem_limit((const void*)attn_fwd_tc_kernel<T, DP, SPLIT>, smem, devices)) return WUBU_B200_ERR_CUDA;
   const long long work = (long long)((a.Tq + 2 * kTile - 1) / (2 * kTile)) * p.splits * a.Hq * a.B;
-  const int sms = attn_sms();
+  const int sms = ops_sms();
   if (work > 0x3FFFFFFF || !sms) return sms ? WUBU_B200_ERR_SHAPE : WUBU_B200_ERR_CUDA;
   attn_fwd_tc_kernel<T, DP, SPLIT><<<(unsigned)(work < sms ? work : sms), kThreads, smem, st>>>(maps, p);
   const int rc = ops_launched("attn_forward");
@@ -518,9 +518,9 @@ int launch_fwd(const AttnFwdMaps& maps, const AttnParams& p, cudaStream_t st) {
 // parts, more than fill the SMs once, 1500 keys 27 / 19.4.)
 int attn_fwd_splits(const WubuB200Attn& a) {
   const long long ctas = (long long)((a.Tq + 2 * kTile - 1) / (2 * kTile)) * a.Hq * a.B;
-  const int tiles = (a.Tk + kTile - 1) / kTile;
-  if (ctas == 0 || ctas > 74) return 1;
-  const long long most = 148 / ctas < kMaxSplits ? 148 / ctas : kMaxSplits;
+  const int tiles = (a.Tk + kTile - 1) / kTile, sms = ops_sms();
+  if (ctas == 0 || 2 * ctas > sms) return 1;
+  const long long most = sms / ctas < kMaxSplits ? sms / ctas : kMaxSplits;
   const int s = (int)(most < tiles ? most : tiles);
   return s > 1 && tiles - (tiles + s - 1) / s > 3 ? s : 1;
 }

@@ -31,6 +31,15 @@ int* ops_status_word() {
   return at[dev];
 }
 
+int ops_sms() {
+  static std::atomic<int> sms[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  n = sms[dev].load();
+  if (!n && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) sms[dev].store(n);
+  return n;
+}
+
 }  // namespace wb
 
 extern "C" int wubu_b200_ops_sync(void* stream) {

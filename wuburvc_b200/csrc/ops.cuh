@@ -11,6 +11,7 @@ namespace wb {
 
 // The operators' device status word (one per device, see wubu_b200_ops_sync); nullptr on a CUDA error.
 int* ops_status_word();
+int ops_sms();  // SMs of the current device; 0 without one
 
 // Raises a kernel's dynamic shared-memory limit, once per device (`devices`: the ones done).
 inline bool ops_smem_limit(const void* kernel, int bytes, std::atomic<uint64_t>& devices) {

@@ -406,7 +406,8 @@ dim3 group_of(int cols) {
 
 // Row ranges of the blocks: as many blocks as run at once (`resident` an SM), within an item.
 ResNormGrid grid_of(const WubuB200ResNorm& a, const dim3& g, int resident) {
-  const long long want = 148 * resident;
+  const int sms = ops_sms();
+  const long long want = (long long)(sms > 0 ? sms : 1) * resident;
   ResNormGrid r{};
   long long per_item = want / a.items;
   const long long most = (a.rows_per_item + g.y - 1) / g.y;

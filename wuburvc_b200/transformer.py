@@ -86,13 +86,17 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
-def _call(what, fn, dev, *args):
-    """fn(*args, current stream of dev) with dev current (the library launches on the current device)."""
+def _on(dev, fn, *args):
+    """fn(*args) with dev current (the library asks and launches on the current device)."""
     if dev == torch.cuda.current_device():
-        rc = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, _raw_stream(dev))
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)
+
+
+def _call(what, fn, dev, *args):
+    """fn(*args, current stream of dev) with dev current."""
+    rc = _on(dev, fn, *args, _raw_stream(dev))
     if rc:
         _check(rc, what)
 
@@ -292,7 +296,7 @@ def resnorm_backward(dr, dh, x, f, *, norm="layer", weight=None, bias=None, post
                                                                   "dbias")), ws, n)
 
     h = L()
-    n = _check(h.wubu_b200_resnorm_workspace(pack(0, 0)), what)
+    n = _check(_on(dev, h.wubu_b200_resnorm_workspace, pack(0, 0)), what)
     ws = x.new_empty(n, dtype=torch.uint8)
     _call(what, h.wubu_b200_resnorm_backward, dev, pack(ws.data_ptr(), n))
     return out
@@ -349,10 +353,10 @@ def _attn_operands(what, q, k, v, causal, window, scale, q_lens, k_lens):
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace(head, backward):
-    """Workspace bytes of a call's sizes (the library's answer depends on nothing else)."""
-    return _check(L().wubu_b200_attn_workspace(_ATTN.pack(*head, 0, 0, *_NO_VIEW * 4, 0, *_NO_VIEW * 4, 0, 0), backward),
-                  "attn_workspace")
+def _workspace(dev, head, backward):
+    """Workspace bytes of a call's sizes on a device (the library's answer depends on those and on its SMs)."""
+    args = _ATTN.pack(*head, 0, 0, *_NO_VIEW * 4, 0, *_NO_VIEW * 4, 0, 0)
+    return _check(_on(dev, L().wubu_b200_attn_workspace, args, backward), "attn_workspace")
 
 
 def attention_forward(q, k, v, *, causal=False, window=0, scale=None, q_lens=None, k_lens=None):
@@ -373,7 +377,7 @@ def attention_forward(q, k, v, *, causal=False, window=0, scale=None, q_lens=Non
     lse = q.new_empty((B, Hq, Tq), dtype=torch.float32)
     body = (*head, *lens, *vq, *vk, *vv, out.data_ptr(), Tq * Hq * D, Hq * D, D, lse.data_ptr(), *_NO_VIEW * 4)
     h = L()
-    n = _workspace(head, 0)
+    n = _workspace(dev, head, 0)
     ws = q.new_empty(n, dtype=torch.uint8) if n else None
     _call(what, h.wubu_b200_attn_forward, dev, _ATTN.pack(*body, _ptr(ws), n))
     return out, lse
@@ -397,7 +401,7 @@ def attention_backward(dout, q, k, v, out, lse, *, causal=False, window=0, scale
     sq, skv = (Tq * Hq * D, Hq * D, D), (Tk * Hkv * D, Hkv * D, D)
     body = (*head, *lens, *vq, *vk, *vv, *vo, lse.data_ptr(), *vg, dq.data_ptr(), *sq, dk.data_ptr(), *skv,
             dv.data_ptr(), *skv)
-    n = _workspace(head, 1)
+    n = _workspace(dev, head, 1)
     ws = q.new_empty(n, dtype=torch.uint8)
     _call(what, L().wubu_b200_attn_backward, dev, _ATTN.pack(*body, ws.data_ptr(), n))
     return dq, dk, dv
