@@ -416,7 +416,9 @@ int wubu_b200_resnorm_backward(const WubuB200ResNorm* a, void* stream);
  * and every stride is a multiple of 8 elements.  lse: fp32 [B][Hq][Tq].  scale: 0 = 1 / sqrt(D).
  * The forward reads q, k, v and writes out, lse; the backward reads those five and dout and writes
  * dq, dk, dv.  Scores, softmax statistics and all sums are fp32; P and dS enter their matrix
- * products in the inputs' type.  The workspace is wubu_b200_attn_workspace bytes (may be 0). */
+ * products in the inputs' type, and rowsum(P dP) is taken as rowsum(dO out) from the rounded out for rows of more than
+ * 16 keys (from the keys in fp32 for others): results are 1.3 to 1.5 times as far off as one rounding of
+ * the exact ones.  The workspace is wubu_b200_attn_workspace bytes (may be 0). */
 typedef struct WubuB200View {
   void* data;
   long long batch, token, head; /* strides in elements */

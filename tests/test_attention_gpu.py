@@ -236,6 +236,55 @@ def test_live_keys_of_no_weight(dtype, D):
     assert (out == 0).all() and (lse == -math.inf).all()
 
 
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 8, 12, 16, 17, 40])
+@pytest.mark.parametrize("mask", [{}, dict(causal=True), dict(window=3), dict(causal=True, window=9)], ids=str)
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+def test_gradients_of_rows_of_few_keys(dtype, D, mask, T):
+    """Error against float64 in units of rounding the exact gradient once.  dQ and dK: that rounding and the one of dS,
+    whose relative size is the same and which their sums average as they average dS itself: sqrt(2) where both
+    spread alike; 1.6 leaves a tenth for the spread over the few elements of short cases (dV: P's, the same).  With D
+    from the 16-bit out two keys are at 2.3 and four to sixteen at 1.7-2."""
+    B = 4096 // T // (D // 32)
+    q, k, v, dout = make(B, 4, 2, T, T, D, dtype, seed=T + D)
+    out, lse = tf.attention_forward(q, k, v, **mask)
+    got = tf.attention_backward(dout, q, k, v, out, lse, **mask)
+    a, b, c = (t.double().transpose(1, 2).requires_grad_(True) for t in (q, k, v))
+    s = (a @ b.repeat_interleave(2, 1).transpose(2, 3)) * D ** -0.5
+    s = s.masked_fill(~visible(T, T, mask.get("causal", False), mask.get("window", 0), T, T), -math.inf)
+    o = torch.softmax(s, -1) @ c.repeat_interleave(2, 1)
+    for x, w in zip(got, torch.autograd.grad(o, (a, b, c), dout.double().transpose(1, 2))):
+        w = w.transpose(1, 2)
+        once = (w.to(dtype).double() - w).norm()
+        assert (x.double() - w).norm() <= (1.6 if T > 1 else 1.0) * once + 1e-6 * w.norm() + 1e-6 * dout.double().norm()
+
+
+@pytest.mark.parametrize("mask", [{}, dict(causal=True), dict(window=20), dict(causal=True, window=5)], ids=str)
+@pytest.mark.parametrize("Tq,Tk", [(70, 40), (33, 50), (90, 12)])
+def test_gradients_of_rows_of_few_keys_with_lengths(Tq, Tk, mask):
+    """The same for items of any length, more and fewer queries than keys, rows that see few keys alone (the others have
+    no gradient to give: their dO is 0)."""
+    B, D = 64, 64
+    q, k, v, dout = make(B, 2, 2, Tq, Tk, D, torch.bfloat16, seed=Tq)
+    g = torch.Generator().manual_seed(Tk)
+    ql, kl = (torch.randint(1, T + 1, (B,), generator=g).int() for T in (Tq, Tk))
+    ql[:8], kl[8:16] = Tq, torch.arange(1, 9)
+    see = torch.stack([visible(Tq, Tk, mask.get("causal", False), mask.get("window", 0), int(m), int(n)) for m, n in zip(ql, kl)])
+    keys = see.sum(-1)
+    few = (keys > 0) & (keys <= 16)
+    dout = dout * few[:, :, None, None]
+    opts = dict(q_lens=ql.cuda(), k_lens=kl.cuda(), **mask)
+    out, lse = tf.attention_forward(q, k, v, **opts)
+    got = tf.attention_backward(dout, q, k, v, out, lse, **opts)
+    a, b, c = (t.double().transpose(1, 2).requires_grad_(True) for t in (q, k, v))
+    s = ((a @ b.transpose(2, 3)) * D ** -0.5).masked_fill(~see[:, None], -1e300)
+    o = torch.softmax(s, -1) @ c
+    for x, w in zip(got, torch.autograd.grad(o, (a, b, c), dout.double().transpose(1, 2))):
+        w = w.transpose(1, 2)
+        once = (w.bfloat16().double() - w).norm()
+        assert (x.double() - w).norm() <= 1.6 * once + 1e-6 * w.norm() + 1e-6 * dout.double().norm()
+
+
 @pytest.mark.parametrize("size", [1e-3, 1.0, 300.0])
 @pytest.mark.parametrize("dtype", list(U), ids=str)
 def test_gradients_of_any_size(size, dtype):

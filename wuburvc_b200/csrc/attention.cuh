@@ -7,7 +7,7 @@ namespace wb {
 struct AttnParams {
   WubuB200Attn a;    // with scale resolved and strides of unit extents cleared
   int group;         // query heads to a key / value head
-  float* delta;      // backward: [B][Hq][t_pad] - rowsum(dO * O)
+  float* delta;      // backward: [B][Hq][t_pad] - rowsum(P * dP)
   float* lse2;       //           the negative log-sum-exp in units of log 2; -infinity where a query sees nothing
   unsigned* counter;    // backward: items drawn
   unsigned* norm_bits;  // backward, fp16: [2][B][Hkv] bits of the largest squared row norms of dO and of V

@@ -1,10 +1,12 @@
 // attention_bwd.cu — the gradient of softmax attention on the tensor cores.
 //
 // With P = 2^(c S - L) recomputed from the scores and the log-sum-exp L (c = scale log2 e, L in units of
-// log 2), D_i = sum_d dO_id O_id and dS = P (dO V^T - D):
+// log 2), D_i = sum_j P_ij (dO V^T)_ij and dS = P (dO V^T - D):
 //   dV = P^T dO,   dK = scale dS^T Q,   dQ = scale dS K.
-// O is the forward's result, rounded to 16 bits: where a row sees few keys that rounding shows in D beside the one
-// of dS (dQ and dK: 1.4 times the error of a single rounding for long rows, 1.5-1.9 for 4 to 16 keys).
+// D is also sum_d dO_id O_id, which takes one pass over the rows where the sum over keys takes two more products.
+// But O is the forward's result, rounded to 16 bits, and where a row sees few keys that rounding shows beside the
+// one of dS (dQ and dK: 2.3 times the error of a single rounding for 2 keys, 1.5-2 for 4 to 16, 1.4 from 32
+// on).  So rows of up to 16 keys sum over them, in float32 (1.3-1.5 times for any length).
 // dK and dV are sums over queries and dQ is a sum over keys.  One grid does both, in two roles: a CTA of the
 // first owns 128 keys and runs over the queries that see them (and over the query heads that share
 // the key head), a CTA of the second owns 128 queries and runs over their keys.  S and dO V^T are formed in
@@ -570,6 +572,7 @@ WB_DEV float dot8(const T* x, const T* y) {
 template <typename T, int N>
 __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnParams p) {
   const WubuB200Attn& a = p.a;
+  griddep_launch();  // (for the kernel of the rows of few keys)
   const int t = threadIdx.x % N, i = blockIdx.x * (256 / N) + threadIdx.x / N, h = blockIdx.y, b = blockIdx.z;
   if (threadIdx.x == 0 && blockIdx.x == 0 && h == 0 && b == 0) *p.counter = 0;
   const AttnItem it(a, b);
@@ -607,6 +610,110 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnParams p) {
       if (vm) atomicMax(p.norm_bits + n + at_, vm);
     }
   }
+}
+
+// Rows of up to kFewKeys keys have their D from the keys.  They lie in the rows [first, last) of an item: any of them
+// where the window is no wider or the item has no more keys, else the 16 rows whose order or window ends at
+// keys 1 to 16.
+constexpr int kFewKeys = 16;
+WB_DEV void few_key_range(const WubuB200Attn& a, const AttnItem& it, int& first, int& last) {
+  first = 0;
+  last = it.ql;
+  if ((a.window > 0 && a.window <= kFewKeys) || it.kl <= kFewKeys) return;
+  const int ahead = a.causal ? 0 : a.window - 1;  // a row at place p sees keys up to p + ahead
+  first = max(0, -ahead - it.off);
+  last = a.causal || a.window > 0 ? min(it.ql, kFewKeys - ahead - it.off) : 0;
+}
+
+// D[16 x 8] += A[16 x 16] B[8 x 16]^T, fragments as mma.sync has them
+WB_DEV void mma_16x8(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, bf16) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+WB_DEV void mma_16x8(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, f16) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// - D of the rows of few keys, over what the kernel before wrote for them; 16 rows to a warp.  Their keys lie within 31 in
+// a row; S and dP are formed 16 x 16 at a time with fragments straight from memory: a tile this small is all
+// latency, and the other tensor path would need it in shared memory first.  The order of a product's values
+// being free, a lane's 8 of every 32 are those that lie together.  Cost (us with / without): 4001 tokens causal, 16
+// heads on 4, 128 values 262 / 260; 16 x 499 causal, 12 heads of 64 76 / 74; with a window of 16 all rows are
+// such: 4 x 4000, 16 heads on 4, 128 values 234 / 189.
+template <typename T>
+__global__ void __launch_bounds__(128) attn_few_keys_kernel(const AttnParams p) {
+  const WubuB200Attn& a = p.a;
+  const int h = blockIdx.y, b = blockIdx.z, warps = blockDim.x / 32;
+  griddep_launch();
+  const AttnItem it(a, b);
+  int start, stop;
+  few_key_range(a, it, start, stop);
+  const int lane = threadIdx.x & 31, g = lane >> 2, t2 = (lane & 3) * 2;
+  const float c = a.scale * kLog2e;
+  bool waited = false;
+  for (int r0 = start + (blockIdx.x * warps + threadIdx.x / 32) * 16; r0 < stop; r0 += gridDim.x * warps * 16) {
+    int lo[2], hi[2], first = a.Tk, end = 0;
+    float l[2], sum[2] = {0.f, 0.f};
+    const T *q[2], *dout[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      int i = r0 + g + 8 * r;
+      lo[r] = it.key_lo(a, i);
+      hi[r] = it.key_hi(a, i);
+      if (hi[r] - lo[r] > kFewKeys) hi[r] = lo[r];  // not one of them
+      if (hi[r] > lo[r]) {
+        first = min(first, lo[r]);
+        end = max(end, hi[r]);
+      }
+      i = min(i, it.ql - 1);  // (beyond the item any row will do)
+      l[r] = a.lse[((long long)b * a.Hq + h) * a.Tq + i] * kLog2e;
+      q[r] = at<T>(a.q, b, i, h) + 4 * t2;
+      dout[r] = at<T>(a.dout, b, i, h) + 4 * t2;
+    }
+    first = __reduce_min_sync(0xffffffffu, first);
+    end = __reduce_max_sync(0xffffffffu, end);
+    for (int j0 = first; j0 < end; j0 += 16) {
+      const T *k[2], *v[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int j = min(j0 + 8 * n + g, end - 1);
+        k[n] = at<T>(a.k, b, j, h / p.group) + 4 * t2;
+        v[n] = at<T>(a.v, b, j, h / p.group) + 4 * t2;
+      }
+      float s[2][4] = {}, dp[2][4] = {};
+#pragma unroll 1
+      for (int d = 0; d < a.D; d += 32) {
+        const bool on = d + 4 * t2 < a.D;
+        auto eight = [&](const T* x) { return on ? __ldg(reinterpret_cast<const uint4*>(x + d)) : make_uint4(0, 0, 0, 0); };
+        const uint4 q0 = eight(q[0]), q1 = eight(q[1]), g0 = eight(dout[0]), g1 = eight(dout[1]);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const uint4 kn = eight(k[n]), vn = eight(v[n]);
+          mma_16x8(s[n], q0.x, q1.x, q0.y, q1.y, kn.x, kn.y, T());
+          mma_16x8(s[n], q0.z, q1.z, q0.w, q1.w, kn.z, kn.w, T());
+          mma_16x8(dp[n], g0.x, g1.x, g0.y, g1.y, vn.x, vn.y, T());
+          mma_16x8(dp[n], g0.z, g1.z, g0.w, g1.w, vn.z, vn.w, T());
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const int n = x >> 2, r = x >> 1 & 1, j = j0 + 8 * n + t2 + (x & 1);
+        if (j >= lo[r] && j < hi[r] && l[r] != -INFINITY) sum[r] += ex2(s[n][x & 3] * c - l[r]) * dp[n][x & 3];
+      }
+    }
+    if (!waited) griddep_wait();
+    waited = true;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+      if (hi[r] > lo[r] && (lane & 3) == 0) p.delta[((long long)b * a.Hq + h) * p.t_pad + r0 + g + 8 * r] = -sum[r];
+    }
+  }
+  if (!waited) griddep_wait();  // what waits for this kernel waits for the one before it too
 }
 
 // A gradient from the float32 sums of its parts, in order; 8 values a thread.
@@ -672,6 +779,14 @@ int launch_bwd(const AttnBwdMaps& maps, const AttnParams& p, int sms, cudaStream
   attn_delta_kernel<T, DP / 8><<<dim3(rows ? (rows + kRows - 1) / kRows : 1, a.Hq, a.B), 256, 0, st>>>(p);
   int rc = ops_launched("attn_backward rows");
   if (rc != WUBU_B200_OK) return rc;
+  // rows of few keys: all may be such, or 16 of an order or a window, or those of short items
+  const bool all_few = (a.window > 0 && a.window <= kFewKeys) || a.Tk <= kFewKeys;
+  if (a.Tq && a.Tk && (all_few || a.causal || a.window || a.k_lens)) {
+    const bool one = !all_few && !a.k_lens;
+    rc = ops_launch_after(attn_few_keys_kernel<T>, dim3(all_few ? p.t_pad / 64 : 1, a.Hq, a.B), dim3(one ? 32 : 128), 0, st,
+                          "attn_backward few keys", p);
+    if (rc != WUBU_B200_OK) return rc;
+  }
   const long long kv = tiles_of(a.Tk) * a.Hkv * a.B * p.kv_splits, qs = tiles_of(a.Tq) * a.Hq * a.B * p.q_splits;
   if (kv + qs > 0x3FFFFFFF) return WUBU_B200_ERR_SHAPE;
   const int work = (int)(kv + qs);

@@ -59,8 +59,10 @@ WB_DEV void mbar_init(uint64_t* bar, uint32_t count) {
 // before its predecessor has finished (the predecessor's CTAs let it in as they exit); it waits here
 // for the predecessor's completion and memory before touching the predecessor's outputs.  A no-op for
 // a kernel launched without the attribute.  (An explicit early trigger in the predecessors measured
-// no faster and slower for the multi-wave kernels, so none is issued.)
+// no faster and slower for the generator's multi-wave kernels, so those issue none.)
 WB_DEV void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets a kernel that was launched to follow this one start once every block of this one has come here or ended.
+WB_DEV void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 WB_DEV void fence_barrier_init() {
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
