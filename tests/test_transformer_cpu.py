@@ -274,3 +274,10 @@ def test_workspaces_are_asked_for_on_the_tensors_device(monkeypatch):
     head = (1, 2, 4, 2, 10, 12, 64, 0, 0, 0.0)
     assert [tf._workspace(dev, head, b) for b in (0, 1) for dev in (1, 0, 1)] == [2000, 1000, 2000, 2001, 1001, 2001]
     tf._workspace.cache_clear()
+
+
+@pytest.mark.parametrize("items,rows", [(1, 0x7FFFFFFF), (0x7FFFFFFF, 1), (1, 0x7FFFFFFF - 12)])
+def test_resnorm_refuses_rows_whose_numbers_would_pass_32_bits(items, rows):
+    """A block adds as many rows as it takes at a time to a row's number."""
+    assert resnorm("workspace", items=items, rows=rows, cols=1, xs=1, fs=1) == SHAPE
+    assert resnorm("workspace", items=1, rows=0x7FFFFF00, cols=1, xs=1, fs=1) > 0

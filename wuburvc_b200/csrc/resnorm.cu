@@ -23,6 +23,8 @@ namespace {
 
 constexpr int kMaxCols = 8192;   // 1024 threads x 8 values
 constexpr int kThreads = 384;    // threads a block, where a row needs no more
+// Rows are numbered in 32 bits: up to 12 are added to a number within the range (as many as a block takes at a time).
+constexpr long long kMaxRows = 0x7FFFFFFFll - 32;
 
 struct RowReduce {  // sums over a row's group of warps; four buffers in turn need one barrier a sum
   float2* buf;      // [4][rows][warps]
@@ -376,7 +378,7 @@ int check_resnorm(const WubuB200ResNorm* a) {
     return WUBU_B200_ERR_ARG;
   if (a->cols < 1 || a->cols > kMaxCols) return WUBU_B200_ERR_SHAPE;
   if (a->items == 0 || a->rows_per_item == 0) return 1;
-  if (a->rows_per_item > 0x7FFFFFFFll / a->items || (a->gate == WUBU_B200_GATE_ITEM && a->items > 65000))
+  if (a->rows_per_item > kMaxRows / a->items || (a->gate == WUBU_B200_GATE_ITEM && a->items > 65000))
     return WUBU_B200_ERR_SHAPE;
   if (!a->x || !a->f || (a->gate && !a->gate_values) || !strides_ok(*a, a->x_stride, a->x) ||
       !strides_ok(*a, a->f_stride, a->f))
