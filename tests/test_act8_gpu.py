@@ -166,6 +166,19 @@ def test_lrelu_sign_of_tiny_blocks(C, dtype):
     assert (again.double() - x.double()).abs().max() <= 2.0 ** -100 and (again[1, :128] == 0).all()
 
 
+def test_parts_of_a_kept_form():
+    """Rows, or whole blocks of columns, of a kept form are a kept form: the same bits as that part of the whole."""
+    x, dy = (torch.randn(3, 40, 512, device="cuda").bfloat16() for _ in range(2))
+    _, kept = tf.act8_forward(x)
+    dx, y = tf.act8_backward(dy, kept, recompute=True)
+    for rows, cols, blocks in ((slice(1, 2), slice(None), slice(None)), (slice(None), slice(128, 384), slice(1, 3))):
+        part = kept._replace(q=kept.q[:, 5:, cols][rows], scale=kept.scale[:, 5:, blocks][rows])
+        dx2, y2 = tf.act8_backward(dy[:, 5:, cols][rows], part, recompute=True)
+        assert torch.equal(dx2, dx[:, 5:, cols][rows]) and torch.equal(y2, y[:, 5:, cols][rows])
+    t = kept._replace(q=kept.q.transpose(0, 1), scale=kept.scale.transpose(0, 1))
+    assert torch.equal(tf.act8_backward(dy.transpose(0, 1), t)[0], dx.transpose(0, 1))
+
+
 def test_empty():
     for shape in ((0, 64), (3, 0)):
         x = torch.empty(shape, device="cuda", dtype=torch.bfloat16)

@@ -281,3 +281,17 @@ def test_resnorm_refuses_rows_whose_numbers_would_pass_32_bits(items, rows):
     """A block adds as many rows as it takes at a time to a row's number."""
     assert resnorm("workspace", items=items, rows=rows, cols=1, xs=1, fs=1) == SHAPE
     assert resnorm("workspace", items=1, rows=0x7FFFFF00, cols=1, xs=1, fs=1) > 0
+
+
+def test_act8_backward_refuses_what_is_no_kept_form():
+    """Scales that do not go with the values would be read past their end."""
+    q, scale = torch.zeros(4, 300, dtype=torch.int8), torch.zeros(4, 3)
+    kept = tf.Kept8(q, scale, "gelu", 0.0, torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA"):
+        tf.act8_backward(None, kept)  # a kept form, on the wrong device
+    for bad in (dict(scale=scale[:3]), dict(scale=scale[:, :2]), dict(scale=scale.double()), dict(q=q.float()), dict(q=q[0]),
+                dict(q=q[:, :128]), dict(dtype=torch.float64), dict(q=q[0, 0])):
+        with pytest.raises(ValueError, match="not a kept form"):
+            tf.act8_backward(None, kept._replace(**bad))
+    with pytest.raises(ValueError, match="act is one of"):
+        tf.act8_backward(None, kept._replace(act="tanh"))

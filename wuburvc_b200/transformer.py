@@ -181,6 +181,13 @@ def act8_backward(dy, kept, recompute=False):
     """``(dx, y)`` from the kept form x' of x: dx = dy act'(x'); y = act(x') if ``recompute``, else
     None.  ``dy=None`` gives ``(None, act(x'))`` alone."""
     q, scale = kept.q, kept.scale
+    if q.dim() < 1 or q.dtype != torch.int8 or scale.dtype != torch.float32 or kept.dtype not in _DTYPES or (
+            scale.shape != (*q.shape[:-1], -(-q.shape[-1] // ACT8_BLOCK))):
+        raise ValueError(f"act8_backward: not a kept form: q {tuple(q.shape)} {q.dtype}, scale {tuple(scale.shape)} "
+                         f"{scale.dtype}, of {kept.dtype}")
+    q, scale = q.contiguous(), scale.contiguous()  # (parts of a kept form may be strided)
+    if kept.act not in _ACTS:
+        raise ValueError(f"act8_backward: act is one of {sorted(_ACTS)}, got {kept.act!r}")
     if dy is not None and (dy.shape != q.shape or dy.dtype != kept.dtype):
         raise ValueError(f"act8_backward: dy is {tuple(q.shape)} {kept.dtype}, got {tuple(dy.shape)} {dy.dtype}")
     dev = _cuda("act8_backward", q, scale, dy)
