@@ -295,3 +295,21 @@ def test_act8_backward_refuses_what_is_no_kept_form():
             tf.act8_backward(None, kept._replace(**bad))
     with pytest.raises(ValueError, match="act is one of"):
         tf.act8_backward(None, kept._replace(act="tanh"))
+
+
+def test_sizes_beyond_32_bits_are_refused(monkeypatch):
+    """2^32 + 64 columns are not 64; what the library is called with is recorded, not called."""
+    calls = []
+    monkeypatch.setattr(tf, "_cuda", lambda what, *ts: 0)
+    monkeypatch.setattr(tf, "_call", lambda *args: calls.append(args))
+    big = 2 ** 32 + 64
+    empty = lambda *s, dtype=torch.bfloat16: torch.empty(s, dtype=dtype, device="meta")  # noqa: E731
+    kept = tf.Kept8(empty(1, big, dtype=torch.int8), empty(1, -(-big // 128), dtype=torch.float32), "gelu", 0.0, torch.bfloat16)
+    for call in (lambda: tf.act8_forward(empty(1, big)), lambda: tf.act8_backward(None, kept),
+                 lambda: tf.resnorm_forward(empty(1, 1, big), empty(1, 1, big)),
+                 lambda: tf.attention_forward(*(empty(1, big, 1, 64),) * 3)):
+        with pytest.raises(ValueError, match="beyond 32 bits"):
+            call()
+    assert not calls
+    for cols in (0x7FFFFFFF, 0x7FFFFFFF - 130):  # to the end of a block they would pass 32 bits
+        assert act8(cols=cols, rows=1) == SHAPE and act8("backward", cols=cols, rows=1) == SHAPE

@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kBlock = 128;        // values that share a scale
 constexpr int kThreads = 256;
+constexpr int kMaxCols = 0x7FFFFFFF - 2 * kBlock;  // columns are numbered in 32 bits, to the end of a block
 constexpr float kTiny = 0x1p-100f;  // below this a block is kept as zeros (127 / max|x| must not overflow), but see block_scale
 
 struct Act8 {
@@ -325,6 +326,7 @@ int check_act8(int dtype, int act, long long rows, int cols) {
   if (!ops_dtype_ok(dtype) || act < WUBU_B200_ACT_IDENTITY || act > WUBU_B200_ACT_LRELU_SIGN) return WUBU_B200_ERR_ARG;
   if (rows < 0 || cols < 0) return WUBU_B200_ERR_ARG;
   if (rows == 0 || cols == 0) return 1;
+  if (cols > kMaxCols) return WUBU_B200_ERR_SHAPE;
   const long long nblk = (cols + kBlock - 1) / kBlock;
   // one warp per block in the general kernels, grid.x below 2^31
   if (rows > (((long long)1 << 31) - 1) * (kThreads / 32) / nblk) return WUBU_B200_ERR_SHAPE;

@@ -86,6 +86,13 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
+def _int32(what, n):
+    """n, a size that the library takes in 32 bits (ctypes would cut it, struct raises an error of its own)."""
+    if n > 2 ** 31 - 1:
+        raise ValueError(f"{what}: a size of {n} is beyond 32 bits")
+    return n
+
+
 def _on(dev, fn, *args):
     """fn(*args) with dev current (the library asks and launches on the current device)."""
     if dev == torch.cuda.current_device():
@@ -167,7 +174,7 @@ def act8_forward(x, act="gelu", slope=0.0, with_output=True):
         raise ValueError("act8_forward: x has a last dimension")
     dev = _cuda("act8_forward", x)
     x, step = _rows(x)
-    C = x.shape[-1]
+    C = _int32("act8_forward", x.shape[-1])
     rows = x.numel() // C if C else 0
     y = _empty(x) if with_output else None
     q = _empty(x, torch.int8)
@@ -191,7 +198,7 @@ def act8_backward(dy, kept, recompute=False):
     if dy is not None and (dy.shape != q.shape or dy.dtype != kept.dtype):
         raise ValueError(f"act8_backward: dy is {tuple(q.shape)} {kept.dtype}, got {tuple(dy.shape)} {dy.dtype}")
     dev = _cuda("act8_backward", q, scale, dy)
-    C = q.shape[-1]
+    C = _int32("act8_backward", q.shape[-1])
     rows = q.numel() // C if C else 0
     step, dx, y = 0, None, None
     if dy is not None:
@@ -236,7 +243,7 @@ def _resnorm_operands(what, x, f, norm, weight, bias, post, post_weight, post_bi
     if (weight is not None and norm is None) or (post_weight is not None and post is None):
         raise ValueError(f"{what}: a weight without its norm")
     dev = _cuda(what, x, f)
-    items, C = x.shape[0], x.shape[-1]
+    items, C = x.shape[0], _int32(what, x.shape[-1])
     rows = x.numel() // (items * C) if items and C else 0
     vec = [v if v is None else _vector(v, (C,), dev, what) for v in (weight, bias, post_weight, post_bias)]
     kind = 0
@@ -355,6 +362,8 @@ def _attn_operands(what, q, k, v, causal, window, scale, q_lens, k_lens):
         raise ValueError(f"{what}: window is not negative, scale is positive")
     dev = _cuda(what, q, k, v)
     ql, kl = _lens(q_lens, B, dev, what), _lens(k_lens, B, dev, what)
+    for n in (B, Hq, Tq, Tk):
+        _int32(what, n)
     head = (d, B, Hq, Hkv, Tq, Tk, D, int(bool(causal)), min(int(window), 2 ** 30), scale or 0.0)
     return dev, head, (_ptr(ql), _ptr(kl)), (ql, kl)
 
