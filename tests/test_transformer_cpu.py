@@ -313,3 +313,12 @@ def test_sizes_beyond_32_bits_are_refused(monkeypatch):
     assert not calls
     for cols in (0x7FFFFFFF, 0x7FFFFFFF - 130):  # to the end of a block they would pass 32 bits
         assert act8(cols=cols, rows=1) == SHAPE and act8("backward", cols=cols, rows=1) == SHAPE
+
+
+@pytest.mark.parametrize("device,want", [(None, 3), ("cuda", 3), (torch.device("cuda"), 3), ("cuda:0", 0), ("cuda:1", 1), (2, 2)])
+def test_ops_sync_waits_on_the_device_it_is_given(device, want, monkeypatch):
+    calls = []
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    monkeypatch.setattr(tf, "_call", lambda what, fn, dev: calls.append(dev))
+    tf.ops_sync(device)
+    assert calls == [want]

@@ -146,7 +146,8 @@ def _rows(t):
 
 def ops_sync(device=None):
     """Waits for the current stream and raises if a kernel of these operators gave up on a wait."""
-    dev = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    dev = None if device is None else torch.device(device).index
+    dev = torch.cuda.current_device() if dev is None else dev
     _call("ops_sync", L().wubu_b200_ops_sync, dev)
 
 
