@@ -122,3 +122,25 @@ def test_autocast():
     assert torch.equal(x.grad, wide[0].grad) and torch.equal(f.grad, wide[1].grad.bfloat16())
     with pytest.raises(ValueError):
         tf.resnorm(x, f)  # outside a region types are the caller's
+
+
+@pytest.mark.parametrize("act,slope", [("lrelu", 0.0), ("lrelu", 0.1), ("lrelu_sign", 0.0), ("gelu", 0.0), ("silu", 0.0)])
+def test_feed_forward_gradients(act, slope):
+    """Against float64's of the function itself, relative L2, float32 operands (products in float32: 1e-6 and a cube root
+    of it for the kink's flips).  The 8-bit form is off by max / 254 / sqrt(3) of a block, 0.7 % of its spread: it
+    enters w2's gradient whole (1.2 % for a ReLU, half of whose values are 0 and whose norm is less) and through
+    act' those of x, w1 and b1, where the leaky ReLU has none.  Differentiated at the rounded value, its own would be off
+    by 7 %."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    leaves = [rnd(300, 64), rnd(512, 64) / 8, 0.1 * rnd(512), rnd(64, 512) / 22, 0.1 * rnd(64)]
+    dout = rnd(300, 64)
+    low = [t.clone().requires_grad_(True) for t in leaves]
+    tf.feed_forward(*low, act=act, slope=slope).backward(dout)
+    x, w1, b1, w2, b2 = high = [t.double().requires_grad_(True) for t in leaves]
+    f = {"gelu": torch.nn.functional.gelu, "silu": torch.nn.functional.silu}.get(
+        act, lambda u: torch.nn.functional.leaky_relu(u, slope))
+    (f(x @ w1.T + b1) @ w2.T + b2).backward(dout.double())
+    off = [float((a.grad.double() - b.grad).norm() / b.grad.norm()) for a, b in zip(low, high)]
+    exact = 1e-3 if act.startswith("lrelu") else 1e-2
+    assert max(off[:3]) < exact and off[3] < 2e-2 and off[4] < 1e-5, off

@@ -165,9 +165,11 @@ class Kept8(NamedTuple):
 
 
 def act8_forward(x, act="gelu", slope=0.0, with_output=True):
-    """``(act(x), kept)``; ``kept`` is what ``act8_backward`` reads in place of x.  ``act``: "lrelu"
-    (with ``slope``; 0 is the ReLU), "gelu", "silu" or "identity"; "lrelu_sign" is the leaky ReLU whose kept
-    positive values stay positive, so that its derivatives are exact.  ``with_output=False`` only keeps x."""
+    """``(act(x), kept)``; ``kept`` is what ``act8_backward`` reads in place of x.  ``act``: "gelu", "silu",
+    "identity", or a leaky ReLU with ``slope`` (0: the ReLU) in one of two forms.  "lrelu_sign" keeps positive values
+    positive: its derivatives are those of x.  "lrelu" rounds like the others and differentiates at the rounded
+    value: what lies within half a step above 0 has the slope's derivative (0.5 % of normally distributed
+    values, a tenth of the gradient's norm).  ``with_output=False`` only keeps x."""
     d = _dtype(x, "act8_forward")
     if act not in _ACTS:
         raise ValueError(f"act8_forward: act is one of {sorted(_ACTS)}, got {act!r}")
@@ -519,5 +521,7 @@ class _FeedForward(torch.autograd.Function):
 
 def feed_forward(x, w1, b1, w2, b2, act="gelu", slope=0.0):
     """act(x w1^T + b1) w2^T + b2, differentiable.  Of its hidden layer the backward keeps the 8-bit form alone: the
-    activation's derivative and the input of w2's gradient are both formed from it.  Under autocast in its type."""
+    activation's derivative and the input of w2's gradient are both formed from it ("lrelu" in the form that keeps
+    signs, so that the derivative is the function's own).  Under autocast in its type."""
+    act = "lrelu_sign" if act == "lrelu" else act
     return _FeedForward.apply(*_autocast(x, w1, b1, w2, b2), act, slope)
