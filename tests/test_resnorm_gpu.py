@@ -153,6 +153,14 @@ def test_zero_rows_and_nan_stay_in_their_row():
     assert (e["dweight"] == 0).all() and (e["dgate"] == 0).all() and e["dgate"].shape == (2, 64)
 
 
+@pytest.mark.parametrize("shape,norm,post,gate", [((2, 1500, 4096), "layer", None, None), ((3, 700, 3200), "rms", "rms", "item"),
+                                                  ((1, 2000, 5001), "layer", "layer", "column")], ids=str)
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+def test_wide_rows_by_the_thousand(shape, dtype, norm, post, gate):
+    """Rows of more than 3072 columns (a block each), many to a block."""
+    check(shape, dtype, norm, post, gate)
+
+
 @pytest.mark.parametrize("C", [96, 97, 4000])
 def test_each_gradient_alone(C):
     """`need` leaves outputs out; what is left has the same bits."""
