@@ -147,6 +147,27 @@ def test_many_padded_items(shape, mask, dtype):
 
 
 @pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_many_calls_in_a_row(D, causal):
+    """A padded batch, back to back and on changing inputs: no wait in the kernels may depend on how late a warp comes to
+    it (steps whose halves are done before the issuing warp looks).  One that did would end after its limit of
+    two seconds and show in ops_sync."""
+    lens = torch.tensor([max(1, 499 - 23 * b) for b in range(16)], dtype=torch.int32, device="cuda")
+    opts = dict(q_lens=lens, k_lens=lens, causal=causal)
+    states = [make(16, 12, 12, 499, 499, D, torch.bfloat16, seed=n) for n in range(3)]
+    kept = [tf.attention_forward(q, k, v, **opts) for q, k, v, _ in states]
+    first = [tf.attention_backward(dout, q, k, v, *o, **opts) for (q, k, v, dout), o in zip(states, kept)]
+    tf.ops_sync()
+    for n in range(600):
+        (q, k, v, dout), o = states[n % 3], kept[n % 3]
+        tf.attention_forward(q, k, v, **opts)
+        grads = tf.attention_backward(dout, q, k, v, *o, **opts)
+        if n % 50 < 3:
+            assert all(torch.equal(a, b) for a, b in zip(grads, first[n % 3]))
+    tf.ops_sync()
+
+
+@pytest.mark.parametrize("D", [64, 128])
 def test_long_sequences(D):
     """Many tiles an item: the rings go round, the running maximum and the sums span 20 tiles."""
     check(*make(1, 4, 1, 2500, 2500, D, torch.bfloat16, seed=D), causal=True)

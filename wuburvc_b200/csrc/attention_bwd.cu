@@ -58,7 +58,7 @@ struct BwdShift<f16> {
 };
 
 struct Barriers {
-  uint64_t item_full[2], item_empty[2], res_full, res_empty, a_full[3], a_empty[3], b_full[kStagesB], b_empty[kStagesB], s_full[2], dp_full, p_ready,
+  uint64_t item_full[2], item_empty[2], res_full, res_empty, a_full[3], a_empty[3], b_full[kStagesB], b_empty[kStagesB], s_full[2], dp_full, p_ready[2],
       ds_ready, acc_full, acc_read, mma_done;
 };
 
@@ -205,7 +205,8 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
     mbar_init(&bar.s_full[0], 1);
     mbar_init(&bar.s_full[1], 1);
     mbar_init(&bar.dp_full, 1);
-    mbar_init(&bar.p_ready, kProducer);
+    mbar_init(&bar.p_ready[0], kProducer);
+    mbar_init(&bar.p_ready[1], kProducer);
     mbar_init(&bar.ds_ready, kProducer);
     mbar_init(&bar.acc_full, 1);
     mbar_init(&bar.acc_read, kProducer);
@@ -284,7 +285,8 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
       const int ksteps = (a.D + 15) / 16;
       const uint64_t dr0 = desc_k(res0), dr1 = desc_k(res1);
       bool ok = true;
-      int n0 = 0, items = 0, p_count = 0;  // steps, items (with steps) and halves of the keys' role so far
+      int n0 = 0, items = 0;           // steps and items (with steps) so far
+      uint32_t p_phase[2] = {0, 0};    // of P, by the buffer of its S
       Items take{bar, item_slots, 0};
       for (BwdWork k; take.take(k, p);) {
         take.done();
@@ -340,11 +342,15 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
         for (int i = 0; i < k.steps; ++i) {
           const int n = n0 + i, sa = n % kA, sb = n % kStagesB;
           if (kv) {
-            if (ok) ok = bar_wait(&bar.p_ready, p_count & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
-            ++p_count;
+            // (with two S the warps may be done with P(i + 1) before this warp looks for P(i): a single barrier, two
+            // phases on, would never show it)
+            const int buf = two_s ? i & 1 : 0;
+            if (ok) ok = bar_wait(&bar.p_ready[buf], buf ? p_phase[1] : p_phase[0], p.err, ERR_WAIT_ACC, p.wait_ns);
+            if (buf) p_phase[1] ^= 1u;
+            else p_phase[0] ^= 1u;
             tc_fence_after();
             if (ok) {
-              issue_acc(tAcc0, tmem + (two_s ? 256 * (i & 1) : 0), rb + sb * kTileBytes, i);
+              issue_acc(tAcc0, tmem + 256 * buf, rb + sb * kTileBytes, i);
               umma_commit_warp(&bar.b_empty[sb]);
             }
             if (!two_s && i + 1 < k.steps) issue_s(i + 1);
@@ -461,7 +467,7 @@ attn_bwd_tc_kernel(const __grid_constant__ AttnBwdMaps maps, const __grid_consta
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bar.p_ready);
+            if (lane == 0) mbar_arrive(&bar.p_ready[buf]);
           }
           ok = bar_wait(&bar.dp_full, (n0 + i) & 1, p.err, ERR_WAIT_ACC, p.wait_ns);
           if (!ok) continue;
