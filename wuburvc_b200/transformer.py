@@ -103,7 +103,11 @@ def _on(dev, fn, *args):
 
 def _call(what, fn, dev, *args):
     """fn(*args, current stream of dev) with dev current."""
-    rc = _on(dev, fn, *args, _raw_stream(dev))
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
     if rc:
         _check(rc, what)
 
@@ -191,17 +195,19 @@ def act8_backward(dy, kept, recompute=False):
     """``(dx, y)`` from the kept form x' of x: dx = dy act'(x'); y = act(x') if ``recompute``, else
     None.  ``dy=None`` gives ``(None, act(x'))`` alone."""
     q, scale = kept.q, kept.scale
-    if q.dim() < 1 or q.dtype != torch.int8 or scale.dtype != torch.float32 or kept.dtype not in _DTYPES or (
-            scale.shape != (*q.shape[:-1], -(-q.shape[-1] // ACT8_BLOCK))):
-        raise ValueError(f"act8_backward: not a kept form: q {tuple(q.shape)} {q.dtype}, scale {tuple(scale.shape)} "
+    shape, blocks, d, act = q.shape, scale.shape, _DTYPES.get(kept.dtype), _ACTS.get(kept.act)
+    if (not shape or q.dtype != torch.int8 or scale.dtype != torch.float32 or d is None or blocks[:-1] != shape[:-1]
+            or len(blocks) != len(shape) or blocks[-1] != -(-shape[-1] // ACT8_BLOCK)):
+        raise ValueError(f"act8_backward: not a kept form: q {tuple(shape)} {q.dtype}, scale {tuple(blocks)} "
                          f"{scale.dtype}, of {kept.dtype}")
-    q, scale = q.contiguous(), scale.contiguous()  # (parts of a kept form may be strided)
-    if kept.act not in _ACTS:
+    if act is None:
         raise ValueError(f"act8_backward: act is one of {sorted(_ACTS)}, got {kept.act!r}")
-    if dy is not None and (dy.shape != q.shape or dy.dtype != kept.dtype):
-        raise ValueError(f"act8_backward: dy is {tuple(q.shape)} {kept.dtype}, got {tuple(dy.shape)} {dy.dtype}")
+    if not (q.is_contiguous() and scale.is_contiguous()):  # parts of a kept form may be strided
+        q, scale = q.contiguous(), scale.contiguous()
+    if dy is not None and (dy.shape != shape or dy.dtype != kept.dtype):
+        raise ValueError(f"act8_backward: dy is {tuple(shape)} {kept.dtype}, got {tuple(dy.shape)} {dy.dtype}")
     dev = _cuda("act8_backward", q, scale, dy)
-    C = _int32("act8_backward", q.shape[-1])
+    C = _int32("act8_backward", shape[-1])
     rows = q.numel() // C if C else 0
     step, dx, y = 0, None, None
     if dy is not None:
@@ -209,7 +215,7 @@ def act8_backward(dy, kept, recompute=False):
         dx = torch.empty_like(q, dtype=kept.dtype)
     if recompute or dy is None:
         y = torch.empty_like(q, dtype=kept.dtype)
-    _call("act8_backward", L().wubu_b200_act8_backward, dev, _DTYPES[kept.dtype], _ACTS[kept.act], kept.slope, _ptr(dy),
+    _call("act8_backward", L().wubu_b200_act8_backward, dev, d, act, kept.slope, _ptr(dy),
           step, q.data_ptr(), scale.data_ptr(), _ptr(dx), _ptr(y), rows, C)
     return dx, y
 
@@ -221,6 +227,7 @@ def act8_restore(kept):
 
 # ---- norms around a block, gate and residual scale ------------------------------------------------
 
+_RESNORM_GRADS = frozenset(("dx", "df", "dgate", "dweight", "dbias", "dpost_weight", "dpost_bias"))
 _RESNORM = struct.Struct("@4i2qi2fi" + "4q" + "4P" + "P" + "2P" + "4q" + "2P" + "5P" + "Pq")
 
 
@@ -302,21 +309,25 @@ def resnorm_backward(dr, dh, x, f, *, norm="layer", weight=None, bias=None, post
     dr, dh = grads
     x, xs = _rows(x)
     f, fs = _rows(f)
-    out = {}
-    for n, v in zip(("dx", "df", "dweight", "dbias", "dpost_weight", "dpost_bias", "dgate"), (x, x, *vec, gate)):
-        out[n] = None if v is None or (need is not None and n not in need) else _empty(v)
+    skip = () if need is None else _RESNORM_GRADS.difference(need)
+    dx = None if "dx" in skip else _empty(x)
+    df = None if "df" in skip else _empty(x)
+    dweight, dbias, dpost_weight, dpost_bias = (None if v is None or n in skip else torch.empty_like(v) for n, v in
+                                                zip(("dweight", "dbias", "dpost_weight", "dpost_bias"), vec))
+    dgate = None if gate is None or "dgate" in skip else torch.empty_like(gate)
 
     def pack(ws, n):
         return _RESNORM.pack(d, _NORMS[norm], _NORMS[post], kind, items, rows, C, res_scale, eps, 0, x.data_ptr(), xs,
                              f.data_ptr(), fs, *map(_ptr, vec), _ptr(gate), 0, 0, _ptr(dr), strides[0], _ptr(dh),
-                             strides[1], *(_ptr(out[m]) for m in ("dx", "df", "dgate", "dpost_weight", "dpost_bias", "dweight",
-                                                                  "dbias")), ws, n)
+                             strides[1], _ptr(dx), _ptr(df), _ptr(dgate), _ptr(dpost_weight), _ptr(dpost_bias),
+                             _ptr(dweight), _ptr(dbias), ws, n)
 
     h = L()
     n = _check(_on(dev, h.wubu_b200_resnorm_workspace, pack(0, 0)), what)
     ws = x.new_empty(n, dtype=torch.uint8)
     _call(what, h.wubu_b200_resnorm_backward, dev, pack(ws.data_ptr(), n))
-    return out
+    return {"dx": dx, "df": df, "dgate": dgate, "dweight": dweight, "dbias": dbias, "dpost_weight": dpost_weight,
+            "dpost_bias": dpost_bias}
 
 
 # ---- attention --------------------------------------------------------------------------------------
@@ -365,8 +376,7 @@ def _attn_operands(what, q, k, v, causal, window, scale, q_lens, k_lens):
         raise ValueError(f"{what}: window is not negative, scale is positive")
     dev = _cuda(what, q, k, v)
     ql, kl = _lens(q_lens, B, dev, what), _lens(k_lens, B, dev, what)
-    for n in (B, Hq, Tq, Tk):
-        _int32(what, n)
+    _int32(what, max(B, Hq, Tq, Tk))
     head = (d, B, Hq, Hkv, Tq, Tk, D, int(bool(causal)), min(int(window), 2 ** 30), scale or 0.0)
     return dev, head, (_ptr(ql), _ptr(kl)), (ql, kl)
 
