@@ -157,7 +157,7 @@ def test_zero_rows_and_nan_stay_in_their_row():
                                                   ((1, 2000, 5001), "layer", "layer", "column")], ids=str)
 @pytest.mark.parametrize("dtype", list(U), ids=str)
 def test_wide_rows_by_the_thousand(shape, dtype, norm, post, gate):
-    """Rows of more than 3072 columns (a block each), many to a block."""
+    """Rows that take a block each, many to a block."""
     check(shape, dtype, norm, post, gate)
 
 

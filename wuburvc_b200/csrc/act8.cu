@@ -8,7 +8,8 @@
 // Both kernels move each byte once: forward 2 + 2 + 1 bytes a 16-bit value,
 // backward 1 + 2 + 2 (+ 2 for y').  Eight threads own a block, 16 values each, as two 16-byte pieces
 // 64 values apart, so that a warp's load covers whole 128-byte lines.  Measured (B200, 7984 x 2048 bf16, GELU):
-// forward 18 us for 82 MB (69 % of the measured copy rate; issue-bound), backward with y' 22 us for 115 MB (79 %).
+// forward 18-20 us for 82 MB (65 % of the measured copy rate; bound by instruction issue: 26 a value, 75 % of the
+// slots), backward with y' 22-24 us for 115 MB (76 %; 25 a value, 57 %, half the warps of an SM).
 #include <type_traits>
 
 #include "ops.cuh"

@@ -23,8 +23,8 @@
 //                           dV(n) | dK(n) dP(n+1) S(n+2)             dS(n) | P(n+1)        up to 64
 //   queries' role:  tensor  dQ(n) dP(n+1) S(n+2)              warps  P(n+1) dS(n+1)
 //
-// Measured (B200): 16 heads on 4, 4001 tokens causal, 128 values: 258 us alone (floor 101 us for 5 products, 141
-// for the 7); 4 x 16 heads, 2048 x 64: 319 us; 16 x up to 499, 12 heads of 64: 72-76 us (floor 9.8).  What bounds
+// Measured (B200): 16 heads on 4, 4001 tokens causal, 128 values: 263 us with its inputs in L2 (floor 101 us for 5
+// products, 141 for the 7); 4 x 16 heads, 2048 x 64: 318 us; 16 x up to 499, 12 heads of 64: 77 us (floor 9.8).  What bounds
 // it is the chain product - exponentials - product of a step: without any exponential it is 5 % faster.
 //
 // fp16 has few small numbers and a low ceiling, so its P is scaled by 2^14 (P <= 1) and its dS by the

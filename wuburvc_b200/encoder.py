@@ -3,7 +3,7 @@
 
 Two forms of layer, over a padded batch x [B, T, width] with lengths:
 
-* ``post`` (the prior encoder's, LayerNorm after each block):
+* ``post`` (LayerNorm after each block, as in the prior encoder, whose relative position terms it leaves out):
       x <- LN(x + attention(x)),  x <- LN(x + feed_forward(x));
 * ``gated`` (norms before and after each block, a gate per item from the speaker embedding g):
       r <- r + gate_a(g) * rms(attention(h)),  h = rms(r),  and the same for the feed-forward.
