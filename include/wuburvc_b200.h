@@ -411,7 +411,8 @@ int wubu_b200_resnorm_backward(const WubuB200ResNorm* a, void* stream);
  * give each item's length: what lies beyond is neither read into a result nor differentiated, and
  * may hold anything.  Query i sits at place p = i + k_len - q_len among the keys; key j is visible
  * if j < k_len, and j <= p (causal), and |p - j| < window (window > 0).  A query that sees no key,
- * or lies beyond q_len, has O = 0, lse = -infinity and no gradient; dk, dv beyond k_len are 0.
+ * or lies beyond q_len, has O = 0, lse = -infinity and no gradient; dk, dv beyond k_len are 0.  A query
+ * with a visible score that is NaN or +infinity has O and lse NaN.
  * dtype: WUBU_B200_BF16 or _F16.  D: a multiple of 8, 8 to 128.  Every pointer is aligned to 16 bytes
  * and every stride is a multiple of 8 elements.  lse: fp32 [B][Hq][Tq].  scale: 0 = 1 / sqrt(D).
  * The forward reads q, k, v and writes out, lse; the backward reads those five and dout and writes

@@ -395,7 +395,8 @@ def attention_forward(q, k, v, *, causal=False, window=0, scale=None, q_lens=Non
     h * Hkv // Hq); ``scale`` defaults to 1 / sqrt(D).  ``q_lens`` / ``k_lens``: int32 ``[B]`` on the device,
     the lengths of padded items (what lies beyond may hold anything).  Query i sits at place
     p = i + k_len - q_len among the keys and sees key j if j < k_len, j <= p (``causal``) and
-    |p - j| < window (``window`` > 0).  A query that sees nothing, or lies beyond q_len, has out 0 and lse -inf."""
+    |p - j| < window (``window`` > 0).  A query that sees nothing, or lies beyond q_len, has out 0 and lse -inf; one
+    with a visible score that is NaN or +infinity has both NaN."""
     what = "attention_forward"
     dev, head, lens, hold = _attn_operands(what, q, k, v, causal, window, scale, q_lens, k_lens)
     q, vq = _view(q)
